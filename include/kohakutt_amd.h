@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define KMI_ABI_VERSION 4
+#define KMI_ABI_VERSION 5
 
 /* Element types of operands. */
 enum kmi_dtype {
@@ -300,6 +300,134 @@ int kmi_layer_norm_bwd(const void* dy, const void* x, const float* mean, const f
                        const void* weight, void* dx, void* dweight, void* dbias, int64_t rows,
                        int64_t width, int32_t x_dtype, int32_t w_dtype, int32_t b_dtype,
                        void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Rotary positions: y = x with the first rotary_dim dims of every head rotated in pairs,
+ *   y1 = scale (x1 cos a - x2 sin a), y2 = scale (x2 cos a + x1 sin a), a = position inv_freq[i],
+ * pair i being dims (i, i + rotary_dim / 2), or (2 i, 2 i + 1) when interleaved; the other
+ * dims are copied.  inverse rotates by -a (the same call is the operator's gradient).
+ * Angles are formed and reduced in 64 bits (positions to 2^53), sines and products in 32,
+ * each value rounded once.  Two tensors (`x[1]` may be NULL) share the positions and one
+ * launch: token (b, s) of [batch, heads, seq, head_dim] tensors, element strides of the
+ * batch, head and seq dims, head-dim stride 1.  positions: int32 or int64 (position_bits),
+ * element (b, s) at b * position_stride[0] + s * position_stride[1].  y may be x itself
+ * with the same strides.  No counterpart among the reference's programs: its fusion covers
+ * RoPE as a pointwise chain (src/kohakutt/fusion).
+ */
+typedef struct kmi_rotary_args {
+    const void* x[2];
+    void* y[2];
+    int64_t heads[2];
+    int64_t x_stride[2][3];
+    int64_t y_stride[2][3];
+    int32_t dtype; /* BF16, F16 or F32 */
+    int32_t interleaved, inverse, position_bits;
+    int64_t batch, seq, head_dim, rotary_dim;
+    const void* positions;
+    int64_t position_stride[2];
+    const float* inv_freq; /* device fp32 [rotary_dim / 2] */
+    double scale;
+} kmi_rotary_args;
+
+int kmi_rotary(const kmi_rotary_args* args, void* stream);
+
+/*
+ * A paged key / value cache: `pages` pages of page_size rows (a multiple of 16) per K/V
+ * head, element (page, head, row, dim) at page * s[0] + head * s[1] + row * s[2] + dim.
+ * Sequence b's key p is row p % page_size of page block_table[b * table_stride + p / page_size];
+ * it holds keys [0, key_lengths[b]), the new tokens of the call being the last of them.
+ *   bits 16: values of `dtype` (BF16 or F16), head dims multiples of 8 up to 256, strides
+ *     multiples of 8 elements, bases 16-byte aligned.
+ *   bits 4: two codes to a byte, the even dim in the low four bits: e2m1 (sign, two
+ *     exponent bits, one mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6), times 2^(scale - 127)
+ *     with one scale byte for 32 dims of a row (255: NaN; 0 for zeros) in k_scale / v_scale; head dims
+ *     multiples of 32 up to 256; code strides (bytes) multiples of 16, bases 16-byte
+ *     aligned.  `dtype` is the type values come out in.
+ * New tokens: cu_seqlens (device int32 [batch + 1] offsets into the `tokens` packed
+ * tokens), or NULL for one token per sequence (tokens == batch).  Token r of sequence b is
+ * key key_lengths[b] - Lq_b + r.  All of block_table, key_lengths and cu_seqlens are
+ * device int32, read in the kernels alone: lengths are clamped into [0, table_width *
+ * page_size], offsets into [0, tokens]; a page outside [0, pages) is page 0 to a reader,
+ * and an append leaves its tokens out, as it does keys at or past that capacity or below 0.
+ */
+typedef struct kmi_paged_cache {
+    void* k;
+    void* v;
+    void* k_scale;
+    void* v_scale;
+    int64_t k_stride[3], v_stride[3], k_scale_stride[3], v_scale_stride[3];
+    int32_t dtype, bits;
+    int64_t pages, page_size, heads_kv, head_dim, head_dim_v;
+    const int32_t* block_table;
+    int64_t table_stride, table_width;
+    const int32_t* key_lengths;
+    const int32_t* cu_seqlens;
+    int64_t batch, tokens;
+} kmi_paged_cache;
+
+/*
+ * Appends new keys and values: k [tokens, heads_kv, head_dim], v [tokens, heads_kv,
+ * head_dim_v] of the cache's dtype (element strides of the token and head dims), k rotated
+ * at its key's position when rotary_dim > 0 (as kmi_rotary), both quantised for 4-bit
+ * caches: per 32 dims the scale 2^(floor(log2 max|x|) - 2), at least 2^-126, codes to nearest
+ * even of x / scale, saturating at 6 (rotated and compared in 64 bits, so codes are those of exact
+ * arithmetic).  q [tokens, heads_q, head_dim] (optional, only with rotary_dim > 0) is rotated
+ * into q_out in the same launch; q_out rows of no sequence are zero.  Tokens of no sequence
+ * write nothing else.  Two tokens of one call for one row: either may stay.
+ */
+typedef struct kmi_paged_append_args {
+    kmi_paged_cache cache;
+    const void* k;
+    const void* v;
+    const void* q;
+    void* q_out;
+    int64_t k_stride[2], v_stride[2], q_stride[2], q_out_stride[2];
+    int64_t heads_q;
+    const float* inv_freq;
+    int64_t rotary_dim;
+    int32_t interleaved;
+    double rotary_scale;
+} kmi_paged_append_args;
+
+int kmi_paged_append(const kmi_paged_append_args* args, void* stream);
+
+/*
+ * Reads a cache back: k_out [batch, heads_kv, max_k, head_dim], v_out [.., head_dim_v]
+ * (contiguous, the cache's dtype, 16-byte aligned), zeros at and past key_lengths[b].
+ * cu_seqlens and tokens are ignored.
+ */
+int kmi_paged_read(const kmi_paged_cache* cache, void* k_out, void* v_out, int64_t max_k, void* stream);
+
+/*
+ * Attention of packed queries over a paged cache: out = softmax(scale q k^T) v, query r of
+ * sequence b seeing keys [0, key_lengths[b]), with causal the first key_lengths[b] - Lq_b +
+ * r + 1 of them (bottom-right); a query that sees no key gets zeros and lse minus infinity,
+ * as do rows of no sequence.  q [tokens, heads_q, head_dim], out [tokens, heads_q, head_dim_v]
+ * (element strides of the token and head dims, as kmi_attn_fwd's), lse optional fp32 natural log
+ * [heads_q, tokens] with strides (head, token).  max_q covers every sequence's new tokens;
+ * max_k sizes the launch (keys past it are still read).  Workspace:
+ * kmi_paged_attn_workspace_bytes, 16-byte aligned, contents free before and after.
+ */
+typedef struct kmi_paged_attn_args {
+    kmi_paged_cache cache;
+    const void* q;
+    void* out;
+    float* lse;
+    int64_t q_stride[2], o_stride[2], lse_stride[2];
+    int64_t heads_q;
+    int64_t max_q, max_k;
+    int32_t causal;
+    double scale;
+} kmi_paged_attn_args;
+
+int kmi_paged_attn_workspace_bytes(const kmi_paged_attn_args* args, size_t* bytes);
+
+/* The kernel a call runs on, a static string: "decode16" or "decode32" (paged_decode_kernel by
+ * rows per K/V head), "tile64" or "tile128" (attn_tile_kernel over pages, by rows per
+ * workgroup).  For tests and profiles. */
+int kmi_paged_attn_kernel(const kmi_paged_attn_args* args, const char** name);
+
+int kmi_paged_attn(const kmi_paged_attn_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 /* The message of the last failed call on this thread ("" if none). */
 const char* kmi_last_error(void);

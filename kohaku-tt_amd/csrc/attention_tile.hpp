@@ -63,8 +63,15 @@ __device__ __forceinline__ float other_half(float v) {
     return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
 }
 
-template <typename T, int DP, int MK, int RG>
-__device__ __forceinline__ void attn_tile(const AttnParams& p, unsigned char* smem, const int bh, const int xt) {
+// Whether a kernel's parameters name a paged cache (paged_tile.hpp): keys are then found
+// through a table, 16 rows of a page at a time, and a workgroup may own a split of them.
+template <typename P>
+inline constexpr bool kPagedKeys = false;
+
+template <typename T, int DP, int MK, int RG, typename P>
+__device__ __forceinline__ void attn_tile(const P& p, unsigned char* smem, const int bh, const int xt,
+                                          const int split = 0) {
+    constexpr bool PAGED = kPagedKeys<P>;
     constexpr int KP = 4 / RG;                       // wavefronts that share a row group
     constexpr int KT = tile_keys(DP, RG), NB = KT / 32 / KP;  // NB: 32-key blocks of a wavefront
     constexpr int ROWS = 32 * RG;
@@ -83,7 +90,18 @@ __device__ __forceinline__ void attn_tile(const AttnParams& p, unsigned char* sm
 
     int q0 = 0, lq = p.seq_q, k0 = 0, lk = p.seq_k;
     int64_t qb = 0, kb = 0, vb = 0, ob = 0, lb = 0;
-    if (p.cu_q) {
+    // Paged keys: the split's first key and the sequence's whole count (lk: the split's).
+    int s0 = 0, lall = 0;
+    if constexpr (PAGED) {
+        const auto span = p.span(seq);
+        q0 = span.q0;
+        lq = min(span.lq, p.seq_q);
+        lall = span.lk;
+        const int per = p.split_keys(lall, KT);
+        s0 = split * per;
+        if (split > 0 && s0 >= lall) return;  // (split 0 writes the rows of a sequence without keys)
+        lk = min(lall - s0, per);
+    } else if (p.cu_q) {
         q0 = min(max(p.cu_q[seq], 0), p.total_q);
         lq = min(min(max(p.cu_q[seq + 1], q0), p.total_q) - q0, p.seq_q);
         k0 = min(max(p.cu_k[seq], 0), p.total_k);
@@ -98,7 +116,7 @@ __device__ __forceinline__ void attn_tile(const AttnParams& p, unsigned char* sm
     }
     const int vrows = lq * G;
     const int r0 = xt * ROWS;
-    if (r0 >= vrows || lk <= 0) return;  // uniform: no barrier has run
+    if (r0 >= vrows || (!PAGED && lk <= 0)) return;  // uniform: no barrier has run
     const int rw0 = r0 + 32 * rg;
     const int row = rw0 + l32;
     const int rr = min(row, vrows - 1);  // rows past the end repeat the last (never written)
@@ -106,7 +124,7 @@ __device__ __forceinline__ void attn_tile(const AttnParams& p, unsigned char* sm
     // keeps the barriers, nothing else.
     const bool live = rw0 < vrows;
     const int pos = fdiv(rr, p.fd_group), head = kvh * G + (rr - pos * G);
-    const int coff = p.cu_q ? lk - lq : 0;
+    const int coff = PAGED ? lall - s0 - lq : (p.cu_q ? lk - lq : 0);
 
     // Q fragments (a negative scale flips their sign, so that c2 is positive; a zero one
     // becomes a c2 that finite scores vanish under and minus infinity does not).
@@ -137,10 +155,18 @@ __device__ __forceinline__ void attn_tile(const AttnParams& p, unsigned char* sm
                                                             static_cast<int64_t>(k0) * p.vs[2]);
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(smem));
     auto request_k = [&](int t, int buf) {
-        TL::request(kbase, kst, t * KT, lk, p.d * ES, okk, wave, lds0 + buf * TILE_B);
+        if constexpr (PAGED)
+            TL::request_pieces([&](int key) { return p.k_rows(seq, kvh, s0 + min(key, lk - 1)); }, kst, t * KT, lk, p.d * ES,
+                               okk, wave, lds0 + buf * TILE_B);
+        else
+            TL::request(kbase, kst, t * KT, lk, p.d * ES, okk, wave, lds0 + buf * TILE_B);
     };
     auto request_v = [&](int t, int buf) {
-        TL::request(vbase, vst, t * KT, lk, p.dv * ES, ovv, wave, lds0 + (2 + buf) * TILE_B);
+        if constexpr (PAGED)
+            TL::request_pieces([&](int key) { return p.v_rows(seq, kvh, s0 + min(key, lk - 1)); }, vst, t * KT, lk, p.dv * ES,
+                               ovv, wave, lds0 + (2 + buf) * TILE_B);
+        else
+            TL::request(vbase, vst, t * KT, lk, p.dv * ES, ovv, wave, lds0 + (2 + buf) * TILE_B);
     };
     // All of vmcnt (the builtin, so that the compiler knows the mask loads are back too).
     auto landed = [&] {
@@ -510,6 +536,24 @@ __device__ __forceinline__ void attn_tile(const AttnParams& p, unsigned char* sm
     const float l = lsum + other_half(lsum);
     if (row >= vrows) return;
     const float inv = l > 0.f ? 1.f / l : 0.f;
+    if constexpr (PAGED) {
+        if (p.split_keys(lall, KT) < lall) {
+            // One of several splits: normalised rows and base-2 log-sum-exps, merged by a launch
+            // of their own.
+            const int64_t at = (static_cast<int64_t>(split) * p.rows_total + q0 + pos) * p.hq + head;
+#pragma unroll
+            for (int b = 0; b < DB; ++b)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int d = 32 * b + 8 * q + 4 * h2;
+                    if (d < p.dv)
+                        *reinterpret_cast<f32x4*>(p.part_o + at * DP + d) =
+                            f32x4{o[b][4 * q] * inv, o[b][4 * q + 1] * inv, o[b][4 * q + 2] * inv, o[b][4 * q + 3] * inv};
+                }
+            if (h2 == 0) p.part_lse[at] = l > 0.f ? m + log2f(l) : -INFINITY;
+            return;
+        }
+    }
     T* dst = static_cast<T*>(p.out) + ob + head * p.os[1] + static_cast<int64_t>(q0 + pos) * p.os[2];
     typedef T t4 __attribute__((ext_vector_type(4)));
 #pragma unroll

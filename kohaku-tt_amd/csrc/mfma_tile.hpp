@@ -132,6 +132,31 @@ struct Tile {
         }
     }
 
+    // The same for rows that lie in pages: each piece of 16 rows starts where `rows_at` (of its
+    // first row) says.
+    template <typename F>
+    static __device__ __forceinline__ void request_pieces(F rows_at, uint32_t stride, int row0, int nrows, int row_bytes,
+                                                          const Offs& off, int wave, uint32_t dst) {
+        if (RW * wave >= TR) return;
+        constexpr int IPP = 16 / RPI;  // instructions of a piece
+        static_assert(RW % 16 == 0 && RPI <= 16, "a wavefront's rows are whole pieces");
+#pragma unroll
+        for (int j = 0; j < RW / 16; ++j) {
+            const int first = row0 + RW * wave + 16 * j;
+            const u32x4 rs = dma_rsrc(rows_at(first), rows_extent(min(16, nrows - first), stride, static_cast<uint32_t>(row_bytes)));
+            const uint32_t at =
+                __builtin_amdgcn_readfirstlane(dst + (RW * wave + 16 * j) * PITCH * static_cast<uint32_t>(sizeof(T)));
+            uint32_t x0 = swz(RW * wave + 16 * j);
+            __asm__ volatile("" : "+s"(x0));
+#pragma unroll
+            for (int i = 0; i < IPP; ++i) {
+                const uint32_t c = 16u * (off.chunk ^ x0 ^ swz(RPI * i));
+                dma16(rs, c < static_cast<uint32_t>(row_bytes) ? off.row + static_cast<uint32_t>(i * RPI) * stride + c : kNoChunk,
+                      at + i * RPI * PITCH * static_cast<uint32_t>(sizeof(T)));
+            }
+        }
+    }
+
     // Lane byte addresses of the operand reads, relative to a tile's first row; tiles start at
     // multiples of a row's bytes, so that a chunk's swizzled place is an XOR of low bits.
     struct Addr {

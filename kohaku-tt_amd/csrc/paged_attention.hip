@@ -1,0 +1,265 @@
+// Attention over a paged cache, host side: argument checks, the launch plan, the merge of key
+// splits and the C ABI entry points.  The kernels are in paged_decode.hpp (at most 32 virtual
+// rows per K/V head) and attention_tile.hpp through paged_tile.hpp (more).
+//
+// A 4-bit cache under the tile kernel is widened once into a dense copy in the workspace
+// (kmi_paged_read's kernel): its rows are read by many row tiles, and the copy's bytes are a few
+// percent of what the products take.
+#include <algorithm>
+#include <cstdlib>
+
+#include "paged_attn.hpp"
+
+namespace kmi {
+namespace paged {
+namespace {
+
+constexpr int kDecodeTile = 32;
+
+struct Plan {
+    bool decode;
+    int rows;        // virtual rows of a workgroup
+    int row_groups;  // tile kernel: 4 or 2
+    int nx;          // row tiles of a unit
+    int splits, min_split;
+    int dp;
+    size_t copy_bytes, part_bytes;
+};
+
+int pad_dim(const kmi_paged_attn_args* a) {
+    return padded_head_dim(std::max(a->cache.head_dim, a->cache.head_dim_v));
+}
+
+// KMI_PAGED_SPLITS=n (read once) pins the key splits.
+int splits_override() {
+    static const int v = [] {
+        const char* e = std::getenv("KMI_PAGED_SPLITS");
+        return e ? std::atoi(e) : 0;
+    }();
+    return v;
+}
+
+int64_t capacity_of(const kmi_paged_attn_args* a) {
+    return std::min(a->cache.table_width * a->cache.page_size, a->max_k);
+}
+
+const char* check_attn(const kmi_paged_attn_args* a) {
+    if (!a) return "null args";
+    if (const char* why = check_cache(a->cache, true)) return why;
+    if (!a->q || !a->out) return "null q or out";
+    if (reinterpret_cast<uintptr_t>(a->q) % 16) return "q must be 16-byte aligned";
+    if (reinterpret_cast<uintptr_t>(a->out) % 8) return "out must be 8-byte aligned";
+    for (int i = 0; i < 2; ++i) {
+        if (a->q_stride[i] % 8) return "q strides must be multiples of 8 elements";
+        if (a->o_stride[i] % 4) return "out strides must be multiples of 4 elements";
+    }
+    if (a->heads_q < 1 || a->heads_q > 65536 || a->heads_q % a->cache.heads_kv) return "heads_kv must divide heads_q";
+    if (a->max_q < 0 || a->max_q > a->cache.tokens) return "max_q must be at most the token count";
+    if (a->max_k < 0) return "max_k must not be negative";
+    if (a->max_q * (a->heads_q / a->cache.heads_kv) > (1 << 30)) return "sizes too large";
+    return nullptr;
+}
+
+Plan make_plan(const kmi_paged_attn_args* a) {
+    Plan pl{};
+    pl.dp = pad_dim(a);
+    const int64_t G = a->heads_q / a->cache.heads_kv;
+    const int64_t vrows = std::max<int64_t>(1, a->max_q * G), units = a->cache.batch * a->cache.heads_kv;
+    const int64_t keys = capacity_of(a);
+    int64_t splits;
+    if (vrows <= 32) {
+        pl.decode = true;
+        pl.rows = vrows <= 16 ? 16 : 32;
+        pl.nx = 1;
+        pl.min_split = 4 * kDecodeTile;
+        splits = ceil_div(1024, std::max<int64_t>(1, units));
+    } else {
+        const int64_t w4 = ceil_div(vrows, 128) * units;
+        pl.row_groups = pl.dp <= 128 && w4 >= 448 ? 4 : 2;
+        pl.rows = 32 * pl.row_groups;
+        pl.nx = static_cast<int>(ceil_div(vrows, pl.rows));
+        pl.min_split = 512;
+        splits = ceil_div(512, std::max<int64_t>(1, pl.nx * units));
+        if (pl.nx * units >= 256) splits = 1;
+    }
+    if (splits_override() > 0) splits = splits_override();
+    pl.splits = static_cast<int>(
+        std::max<int64_t>(1, std::min<int64_t>({splits, int64_t{kMaxSplits}, ceil_div(keys, pl.min_split)})));
+    if (a->cache.bits == 4 && !pl.decode)
+        pl.copy_bytes = static_cast<size_t>(units) * keys * (a->cache.head_dim + a->cache.head_dim_v) * 2;
+    if (pl.splits > 1)
+        pl.part_bytes = static_cast<size_t>(pl.splits) * a->cache.tokens * a->heads_q * (pl.dp + 4) * sizeof(float);
+    return pl;
+}
+
+// One wavefront per (query token, query head) of a split sequence: the splits' normalised rows
+// weighted by their sums.
+template <typename T, int DP>
+__global__ __launch_bounds__(kWave) void merge_kernel(const AttnParams p, const int unit_keys, const int row_blocks) {
+    constexpr int E = DP <= 64 ? 1 : (DP <= 128 ? 2 : 4);  // dims of a lane (value head dims are multiples of 8)
+    const int bh = blockIdx.x / row_blocks, r = blockIdx.x - bh * row_blocks;
+    const int seq = fwd::fdiv(bh, p.fd_hkv), kvh = bh - seq * p.hkv;
+    const Span sp = p.span(seq);
+    if (r >= min(sp.lq, p.seq_q) * p.group) return;
+    const int per = p.split_keys(sp.lk, unit_keys);
+    if (per >= sp.lk) return;  // one split: its workgroup wrote the output
+    const int n = (sp.lk + per - 1) / per;
+    const int pos = fwd::fdiv(r, p.fd_group), head = kvh * p.group + (r - pos * p.group);
+    const int64_t tok = sp.q0 + pos, row = tok * p.hq + head, step = p.rows_total * p.hq;
+    const int lane = threadIdx.x, d0 = lane * E;
+    const float lse = lane < n ? p.part_lse[lane * step + row] : -INFINITY;
+    const float top = wave_max(lse);
+    const float w = lse == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(lse - top);
+    const float total = wave_sum(w);
+    const float inv = total > 0.f ? 1.f / total : 0.f;
+    float acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    if (d0 < p.dv) {
+        const float* src = p.part_o + row * DP + d0;
+#pragma unroll 8
+        for (int s = 0; s < n; ++s) {
+            const float ws = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), s));
+            float x[E];
+            __builtin_memcpy(x, __builtin_assume_aligned(src + s * step * DP, E * 4), E * 4);
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] += ws * x[e];
+        }
+        T y[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] = from_f32<T>(acc[e] * inv);
+        T* dst = static_cast<T*>(p.out) + head * p.os[1] + tok * p.os[2] + d0;
+        __builtin_memcpy(__builtin_assume_aligned(dst, E * 2), y, E * 2);
+    }
+    if (p.lse && lane == 0)
+        p.lse[head * p.ls[1] + tok * p.ls[2]] = total > 0.f ? (top + log2f(total)) * 0.6931471805599453f : -INFINITY;
+}
+
+template <typename T, int DP>
+hipError_t run(const AttnParams& p, const Plan& pl, bool four, hipStream_t stream) {
+    const hipError_t err = pl.decode ? launch_decode<T, DP>(p, pl.rows, four, stream)
+                                     : launch_tile<T, DP>(p, pl.row_groups, stream);
+    if (err != hipSuccess || pl.splits == 1) return err;
+    // (The tile kernel's key tiles: 128 for two row groups up to head dim 64, else 64.)
+    const int unit = pl.decode ? kDecodeTile : (DP <= 64 && pl.row_groups == 2 ? 128 : 64);
+    const int rows = p.seq_q * p.group;
+    hipLaunchKernelGGL((merge_kernel<T, DP>), dim3(static_cast<unsigned>(p.batch * p.hkv * rows)), dim3(kWave), 0, stream, p,
+                       unit, rows);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t run_dim(const AttnParams& p, const Plan& pl, bool four, hipStream_t stream) {
+    switch (pl.dp) {
+        case 32: return run<T, 32>(p, pl, four, stream);
+        case 64: return run<T, 64>(p, pl, four, stream);
+        case 96: return run<T, 96>(p, pl, four, stream);
+        case 128: return run<T, 128>(p, pl, four, stream);
+        case 192: return run<T, 192>(p, pl, four, stream);
+        default: return run<T, 256>(p, pl, four, stream);
+    }
+}
+
+// Launches hold fewer than 2^32 threads; 32-bit workgroup arithmetic fits below that.
+bool grid_fits(const kmi_paged_attn_args* a, const Plan& pl) {
+    const double units = static_cast<double>(a->cache.batch) * a->cache.heads_kv;
+    const double blocks = units * pl.nx * pl.splits;
+    const double rows = pl.splits > 1 ? units * a->max_q * (a->heads_q / a->cache.heads_kv) : 0.0;
+    return blocks < (1 << 24) - 1 && rows < (1 << 26);
+}
+
+}  // namespace
+}  // namespace paged
+}  // namespace kmi
+
+extern "C" int kmi_paged_attn_workspace_bytes(const kmi_paged_attn_args* a, size_t* bytes) {
+    using namespace kmi;
+    if (!bytes) return fail(KMI_EINVAL, "kmi_paged_attn_workspace_bytes: null bytes");
+    if (const char* why = paged::check_attn(a))
+        return fail(KMI_EINVAL, std::string("kmi_paged_attn_workspace_bytes: ") + why);
+    const paged::Plan pl = paged::make_plan(a);
+    *bytes = pl.copy_bytes + pl.part_bytes;
+    return KMI_OK;
+}
+
+extern "C" int kmi_paged_attn_kernel(const kmi_paged_attn_args* a, const char** name) {
+    using namespace kmi;
+    if (!name) return fail(KMI_EINVAL, "kmi_paged_attn_kernel: null name");
+    if (const char* why = paged::check_attn(a)) return fail(KMI_EINVAL, std::string("kmi_paged_attn_kernel: ") + why);
+    const paged::Plan pl = paged::make_plan(a);
+    *name = pl.decode ? (pl.rows == 16 ? "decode16" : "decode32") : (pl.row_groups == 4 ? "tile128" : "tile64");
+    return KMI_OK;
+}
+
+extern "C" int kmi_paged_attn(const kmi_paged_attn_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+    using namespace kmi;
+    using namespace kmi::paged;
+    if (const char* why = check_attn(a)) return fail(KMI_EINVAL, std::string("kmi_paged_attn: ") + why);
+    if (a->cache.tokens == 0 || a->cache.batch == 0) return KMI_OK;
+    const Plan pl = make_plan(a);
+    const size_t need = pl.copy_bytes + pl.part_bytes;
+    if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
+        return fail(KMI_EWORKSPACE,
+                    "kmi_paged_attn: workspace missing, misaligned or smaller than kmi_paged_attn_workspace_bytes");
+    if (!grid_fits(a, pl)) return fail(KMI_EINVAL, "kmi_paged_attn: too many workgroups");
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const int64_t keys = capacity_of(a);
+    AttnParams p{};
+    p.c = device_cache(a->cache);
+    p.c.capacity = static_cast<int>(keys);
+    const bool copy = pl.copy_bytes > 0;
+    if (copy) {
+        if (!read_fits(a->cache, keys)) return fail(KMI_EINVAL, "kmi_paged_attn: max_k out of range");
+        const int64_t units = a->cache.batch * a->cache.heads_kv;
+        char* const kc = static_cast<char*>(workspace);
+        char* const vc = kc + static_cast<size_t>(units) * keys * a->cache.head_dim * 2;
+        const hipError_t err = launch_read(a->cache, kc, vc, keys, s);
+        if (err != hipSuccess) return hip_status(err, "kmi_paged_attn");
+        p.head_pages = 1;
+        p.c.k = kc;
+        p.c.v = vc;
+        const int64_t d[2] = {a->cache.head_dim, a->cache.head_dim_v};
+        for (int w = 0; w < 2; ++w) {
+            int64_t* st = w ? p.c.vs : p.c.ks;
+            st[2] = d[w] * 2;
+            st[1] = keys * st[2];
+            st[0] = a->cache.heads_kv * st[1];
+        }
+    }
+    p.q = a->q;
+    p.out = a->out;
+    p.lse = a->lse;
+    p.qs[1] = a->q_stride[1];
+    p.qs[2] = a->q_stride[0];
+    p.os[1] = a->o_stride[1];
+    p.os[2] = a->o_stride[0];
+    p.ls[1] = a->lse_stride[0];
+    p.ls[2] = a->lse_stride[1];
+    // (The tile kernel takes row strides in elements.)
+    p.ks[2] = p.c.ks[2] / 2;
+    p.vs[2] = p.c.vs[2] / 2;
+    p.batch = static_cast<int>(a->cache.batch);
+    p.hq = static_cast<int>(a->heads_q);
+    p.hkv = static_cast<int>(a->cache.heads_kv);
+    p.group = p.hq / p.hkv;
+    p.seq_q = static_cast<int>(a->max_q);
+    p.d = static_cast<int>(a->cache.head_dim);
+    p.dv = static_cast<int>(a->cache.head_dim_v);
+    p.causal = a->causal ? 1 : 0;
+    p.scale_log2 = static_cast<float>(a->scale * 1.4426950408889634);
+    p.splits = pl.splits;
+    p.min_split = pl.min_split;
+    p.nx = pl.nx;
+    p.rows_total = a->cache.tokens;
+    p.fd_splits = fwd::fast_div(static_cast<uint32_t>(p.splits));
+    p.fd_units = fwd::fast_div(static_cast<uint32_t>(p.batch * p.hkv));
+    p.fd_hkv = fwd::fast_div(static_cast<uint32_t>(p.hkv));
+    p.fd_group = fwd::fast_div(static_cast<uint32_t>(p.group));
+    if (pl.splits > 1) {
+        p.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.copy_bytes);
+        p.part_lse = p.part_o + static_cast<size_t>(pl.splits) * p.rows_total * p.hq * pl.dp;
+    }
+    const bool four = a->cache.bits == 4;
+    const hipError_t err = a->cache.dtype == KMI_BF16 ? run_dim<bf16>(p, pl, four, s) : run_dim<f16>(p, pl, four, s);
+    return hip_status(err, "kmi_paged_attn");
+}

@@ -1,0 +1,481 @@
+// Attention over a paged cache for few query rows: single tokens and short drafts, at most 32
+// "virtual rows" (query tokens x GQA group) per (sequence, K/V head).
+//
+// Bound by the cache's bytes.  A unit's keys are split over workgroups and dealt to their four
+// wavefronts in tiles of 32, each tile two halves of 16 rows that lie in one page each (page
+// sizes are multiples of 16), read through a buffer resource of their own: rows past the last key
+// read as zeros, so nothing stale in a page is ever touched.  The wavefronts share nothing until
+// the end and so need no barrier: K goes straight into MFMA operand registers, V through a
+// private LDS tile read transposed; the next tile's loads and the table entries of the one after
+// are in flight during a tile's arithmetic.  S^T = K Q^T leaves a query row per lane, its
+// softmax state is scalar; P feeds O^T += V^T P^T as it stands.
+//
+// 16-bit caches: 16x16x32 MFMAs.  4-bit caches: the codes of K are the operand of the scaled
+// 16x16x128 MFMA as they lie in memory, with the cache's own scale bytes; no key is ever
+// widened.  Its other operand, Q, is the sum of two (bf16) or three (fp16) e4m3 parts of four
+// significant bits, 2^-4 apart, on one power of two per row: bf16's eight bits fit two parts
+// exactly (elements below 2^-13 of the row's largest to within 2^-17 of it), fp16's eleven fit
+// three.  V's codes are widened by the packed conversions on their way into the LDS tile.
+#pragma once
+
+#include "paged_attn.hpp"
+
+namespace kmi {
+namespace paged {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+template <typename T>
+struct Mfma16;
+template <>
+struct Mfma16<bf16> {
+    typedef bf16x8 v8;
+    static __device__ __forceinline__ f32x4 run(v8 a, v8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+};
+template <>
+struct Mfma16<f16> {
+    typedef f16x8 v8;
+    static __device__ __forceinline__ f32x4 run(v8 a, v8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+};
+
+// gfx950's transposed LDS read (see mfma_tile.hpp).
+template <typename T>
+__device__ __forceinline__ u32x2 tr_read(const T* p) {
+    if constexpr (std::is_same<T, bf16>::value) {
+        typedef __attribute__((__vector_size__(4 * sizeof(__bf16)))) __bf16 x4;
+        return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+                                             (__attribute__((address_space(3))) x4*)(reinterpret_cast<uintptr_t>(p))));
+    } else {
+        typedef __attribute__((__vector_size__(4 * sizeof(__fp16)))) __fp16 x4;
+        return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4f16(
+                                             (__attribute__((address_space(3))) x4*)(reinterpret_cast<uintptr_t>(p))));
+    }
+}
+
+// Reductions over the four lanes that hold a row (lane, lane ^ 16, lane ^ 32, lane ^ 48).
+__device__ __forceinline__ float max4(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float sum4(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+constexpr int WAVES = 4;
+constexpr int THREADS = WAVES * kWave;
+constexpr int TK = 32;                // keys of a tile
+constexpr float kLazy = 8.f;          // log2 units a row max may grow before O is rescaled
+constexpr float kLn2f = 0.6931471805599453f;
+constexpr uint32_t kNone = 0x80000000u;  // an offset past every range: reads as zeros
+
+// Parts of a 4-bit call's Q.
+template <typename T>
+constexpr int kParts = std::is_same<T, bf16>::value ? 2 : 3;
+
+// LDS row pitch of the V tile: 16 elements of padding spread the rows over the banks.
+constexpr int v_pitch(int dp) { return dp + 16; }
+
+template <typename T, int DP, int NQ>
+constexpr size_t decode_lds() {
+    const size_t v = static_cast<size_t>(WAVES) * TK * v_pitch(DP) * sizeof(T);
+    const size_t merge = static_cast<size_t>(2) * NQ * 16 * (DP + 4) * sizeof(float) + 2 * NQ * 16 * 2 * sizeof(float);
+    return v > merge ? v : merge;
+}
+
+template <typename T, int DP, int NQ, bool FOUR>
+__global__ __launch_bounds__(THREADS) void paged_decode_kernel(const AttnParams p) {
+    typedef typename Mfma16<T>::v8 v8;
+    constexpr int DC = DP / 32;                // K fragments of a key row (16 bits)
+    constexpr int KC = (DP + 127) / 128;       // the same at 4 bits
+    constexpr int DB = DP / 16;                // output blocks
+    constexpr int VP = v_pitch(DP);
+    constexpr int CP = DP + 4;
+    // V staging, 16 bits: VPS lanes a row (a power of two; those past the padded row idle).
+    constexpr int NCH = DP / 8;
+    constexpr int VPS = NCH <= 4 ? 4 : NCH <= 8 ? 8 : NCH <= 16 ? 16 : 32;
+    constexpr int RPP = kWave / VPS, KIT = 16 / RPP;  // rows a pass, passes of a half
+    // V staging, 4 bits: chunks of 32 dims (one scale byte), N4 a row, R4 rounds of a half.
+    constexpr int N4 = DP / 32, R4 = (16 * N4 + kWave - 1) / kWave;
+
+    extern __shared__ __align__(16) unsigned char smem[];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g4 = lane >> 4, l16 = lane & 15;
+    const int units = p.batch * p.hkv;
+    if (static_cast<int>(blockIdx.x) == units * p.splits) {
+        zero_tail<T>(p);
+        return;
+    }
+    const int bh = fwd::fdiv(static_cast<int>(blockIdx.x), p.fd_splits);
+    const int split = blockIdx.x - bh * p.splits;
+    const int seq = fwd::fdiv(bh, p.fd_hkv), kvh = bh - seq * p.hkv;
+    const int G = p.group;
+    const Span sp = p.span(seq);
+    const int vrows = min(min(sp.lq, p.seq_q) * G, 16 * NQ);
+    const int lk = sp.lk;
+    const int per = p.split_keys(lk, TK);
+    // (Uniform.)  Split 0 writes the rows of a sequence without keys.
+    if (vrows <= 0 || (split > 0 && split * per >= lk)) return;
+    const bool alone = per >= lk;
+    const int t0 = split * (per / TK), t1 = min((lk + TK - 1) / TK, t0 + per / TK);
+
+    // This lane's rows: query position and head, and the keys they see.
+    int pos[NQ], head[NQ], lim[NQ];
+    bool valid[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int r = 16 * n + l16;
+        valid[n] = r < vrows;
+        const int rr = valid[n] ? r : 0;
+        pos[n] = fwd::fdiv(rr, p.fd_group);
+        head[n] = kvh * G + (rr - pos[n] * G);
+        lim[n] = p.causal ? min(lk, lk - sp.lq + pos[n] + 1) : lk;
+    }
+    // A negative scale flips Q's sign, so that the row maximum of the products is that of the
+    // logits; a zero one becomes a factor that finite products vanish under.
+    const float c2 = fmaxf(fabsf(p.scale_log2), 1e-30f);
+    const bool flip = p.scale_log2 < 0.f;
+    auto q_row = [&](int n) {
+        return static_cast<const T*>(p.q) + head[n] * p.qs[1] + static_cast<int64_t>(sp.q0 + pos[n]) * p.qs[2];
+    };
+    v8 qf[FOUR ? 1 : NQ][FOUR ? 1 : DC];
+    i32x8 q8[FOUR ? NQ : 1][FOUR ? KC : 1][FOUR ? kParts<T> : 1];
+    int qsc[FOUR ? NQ : 1];  // scale byte of the first part
+    if constexpr (!FOUR) {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int c = 0; c < DC; ++c) {
+                const int col = 32 * c + 8 * g4;
+                const u32x4 x = *reinterpret_cast<const u32x4*>(q_row(n) + min(col, p.d - 8)) ^ (flip ? 0x80008000u : 0u);
+                qf[n][c] = __builtin_bit_cast(v8, col < p.d ? x : u32x4{0u, 0u, 0u, 0u});
+            }
+    } else {
+        // The scaled MFMA's B operand: bytes 0 .. 15 of lane (g4, l16) are dims 16 g4 .., bytes
+        // 16 .. 31 dims 64 + 16 g4 .. of its 128.
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            v8 x[KC][4];
+            float top = 0.f;
+#pragma unroll
+            for (int c = 0; c < KC; ++c)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int col = 128 * c + 64 * (j >> 1) + 16 * g4 + 8 * (j & 1);
+                    const u32x4 raw = *reinterpret_cast<const u32x4*>(q_row(n) + min(col, p.d - 8));
+                    x[c][j] = __builtin_bit_cast(v8, col < p.d ? raw : u32x4{0u, 0u, 0u, 0u});
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(to_f32(x[c][j][e])));
+                }
+            top = max4(top);
+            // 2^(E - 7), E the exponent of the row's largest: parts below 256 in magnitude.
+            const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 7, 16), 240);
+            qsc[n] = e;
+            const float inv = __uint_as_float(static_cast<uint32_t>(254 - e) << 23) * (flip ? -1.f : 1.f);
+#pragma unroll
+            for (int c = 0; c < KC; ++c)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float y[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) y[i] = to_f32(x[c][j][i]) * inv;
+#pragma unroll
+                    for (int w = 0; w < kParts<T>; ++w) {
+#pragma unroll
+                        for (int i = 0; i < 8; i += 4) {
+                            int b = __builtin_amdgcn_cvt_pk_fp8_f32(y[i], y[i + 1], 0, false);
+                            b = __builtin_amdgcn_cvt_pk_fp8_f32(y[i + 2], y[i + 3], b, true);
+                            q8[n][c][w][2 * j + i / 4] = b;
+                            y[i] = 16.f * (y[i] - __builtin_amdgcn_cvt_f32_fp8(b, 0));
+                            y[i + 1] = 16.f * (y[i + 1] - __builtin_amdgcn_cvt_f32_fp8(b, 1));
+                            y[i + 2] = 16.f * (y[i + 2] - __builtin_amdgcn_cvt_f32_fp8(b, 2));
+                            y[i + 3] = 16.f * (y[i + 3] - __builtin_amdgcn_cvt_f32_fp8(b, 3));
+                        }
+                    }
+                }
+        }
+    }
+
+    // A tile in registers.
+    v8 kreg[FOUR ? 1 : 2][FOUR ? 1 : DC];
+    u32x4 vreg[FOUR ? 1 : 2][FOUR ? 1 : KIT];
+    u32x4 k4[FOUR ? 2 : 1][FOUR ? KC : 1], v4[FOUR ? 2 : 1][FOUR ? R4 : 1];
+    uint32_t k4s[FOUR ? 2 : 1][FOUR ? KC : 1], v4s[FOUR ? 2 : 1][FOUR ? R4 : 1];
+    T* const vl = reinterpret_cast<T*>(smem) + wave * TK * VP;
+    const int krow = lane / VPS, dg = lane % VPS;
+    const uint32_t kst = static_cast<uint32_t>(p.c.ks[2]), vst = static_cast<uint32_t>(p.c.vs[2]);
+
+    // Table entries of a tile's halves (keys past the last one repeat its page).
+    struct Entry {
+        int page[2], row[2];
+    };
+    auto entries = [&](int t) {
+        Entry e;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) e.page[h] = p.page_at(seq, min(TK * t + 16 * h, lk - 1), e.row[h]);
+        return e;
+    };
+    auto load_tile = [&](int t, const Entry& e) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int rows = min(lk - TK * t - 16 * h, 16);
+            const char* kb = p.c.k + e.page[h] * p.c.ks[0] + kvh * p.c.ks[1] + e.row[h] * p.c.ks[2];
+            const char* vb = p.c.v + e.page[h] * p.c.vs[0] + kvh * p.c.vs[1] + e.row[h] * p.c.vs[2];
+            if constexpr (!FOUR) {
+                const auto rk = buffer_rsrc(kb, rows_extent(rows, kst, 2 * p.d));
+                const auto rv = buffer_rsrc(vb, rows_extent(rows, vst, 2 * p.dv));
+#pragma unroll
+                for (int c = 0; c < DC; ++c)
+                    kreg[h][c] = __builtin_bit_cast(
+                        v8, buffer_load16(rk, 32 * c + 8 * g4 < p.d ? l16 * kst + 16 * g4 + 64 * c : kNone));
+#pragma unroll
+                for (int i = 0; i < KIT; ++i)
+                    vreg[h][i] = buffer_load16(rv, 8 * dg < p.dv ? (krow + i * RPP) * vst + 16 * dg : kNone);
+            } else {
+                const uint8_t* ksb = p.c.ksc + e.page[h] * p.c.kss[0] + kvh * p.c.kss[1] + e.row[h] * p.c.kss[2];
+                const uint8_t* vsb = p.c.vsc + e.page[h] * p.c.vss[0] + kvh * p.c.vss[1] + e.row[h] * p.c.vss[2];
+                const uint32_t kss = static_cast<uint32_t>(p.c.kss[2]), vss = static_cast<uint32_t>(p.c.vss[2]);
+                const auto rk = buffer_rsrc(kb, rows_extent(rows, kst, p.d / 2));
+                const auto rv = buffer_rsrc(vb, rows_extent(rows, vst, p.dv / 2));
+                const auto rks = buffer_rsrc(ksb, rows_extent(rows, kss, p.d / 32));
+                const auto rvs = buffer_rsrc(vsb, rows_extent(rows, vss, p.dv / 32));
+#pragma unroll
+                for (int c = 0; c < KC; ++c) {
+                    const bool in = 128 * c + 32 * g4 < p.d;
+                    k4[h][c] = buffer_load16(rk, in ? l16 * kst + 64 * c + 16 * g4 : kNone);
+                    k4s[h][c] = __builtin_amdgcn_raw_buffer_load_b8(rks, in ? l16 * kss + 4 * c + g4 : kNone, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < R4; ++i) {
+                    const int ci = lane + kWave * i, r = ci / N4, ch = ci % N4;
+                    const bool in = r < 16 && 32 * ch < p.dv;
+                    v4[h][i] = buffer_load16(rv, in ? r * vst + 16 * ch : kNone);
+                    v4s[h][i] = __builtin_amdgcn_raw_buffer_load_b8(rvs, in ? r * vss + ch : kNone, 0, 0);
+                }
+            }
+        }
+    };
+    // The tile's V rows into the wavefront's LDS.
+    auto stage = [&] {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if constexpr (!FOUR) {
+                if (dg < NCH) {
+#pragma unroll
+                    for (int i = 0; i < KIT; ++i)
+                        *reinterpret_cast<u32x4*>(vl + (16 * h + krow + i * RPP) * VP + 8 * dg) = vreg[h][i];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < R4; ++i) {
+                    const int ci = lane + kWave * i, r = ci / N4, ch = ci % N4;
+                    if (16 * N4 % kWave != 0 && r >= 16) continue;
+                    const float s = scale_of(v4s[h][i]);
+                    T* dst = vl + (16 * h + r) * VP + 32 * ch;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        u32x4 w;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) w[e] = fp4_pair<T>(v4[h][i][j], s, e);
+                        *reinterpret_cast<u32x4*>(dst + 8 * j) = w;
+                    }
+                }
+            }
+        }
+    };
+
+    f32x4 o[NQ][DB];
+    float m[NQ], thr[NQ], neg_m[NQ], lsum[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+        m[n] = thr[n] = -INFINITY;
+        neg_m[n] = lsum[n] = 0.f;
+    }
+
+    int t = t0 + wave;
+    Entry next{};
+    if (t < t1) {
+        const Entry first = entries(t);
+        if (t + WAVES < t1) next = entries(t + WAVES);
+        load_tile(t, first);
+    }
+    for (; t < t1; t += WAVES) {
+        // LDS keeps one wavefront's accesses in order (the previous tile's reads, these writes,
+        // this tile's reads): only the compiler must keep it.
+        __asm__ volatile("" ::: "memory");
+        stage();
+        f32x4 s[NQ][2];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                s[n][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if constexpr (!FOUR) {
+#pragma unroll
+                    for (int c = 0; c < DC; ++c) s[n][h] = Mfma16<T>::run(kreg[h][c], qf[n][c], s[n][h]);
+                } else {
+#pragma unroll
+                    for (int w = 0; w < kParts<T>; ++w)
+#pragma unroll
+                        for (int c = 0; c < KC; ++c) {
+                            const i32x4 a = __builtin_bit_cast(i32x4, k4[h][c]);
+                            // (Format 4: e2m1, its operand in the first four registers; 0: e4m3.)
+                            s[n][h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                                __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1), q8[n][c][w], s[n][h], 4, 0, 0,
+                                static_cast<int>(k4s[h][c]), 0, qsc[n] - 4 * w);
+                        }
+                }
+            }
+        // The K operands are consumed: the next tile's loads overlap the softmax and PV.
+        if (t + WAVES < t1) {
+            load_tile(t + WAVES, next);
+            if (t + 2 * WAVES < t1) next = entries(t + 2 * WAVES);
+        }
+        v8 pf[NQ];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            // Lane (g4, l16), register i of half h: key 16 h + 4 g4 + i of row l16.
+            const int rel = lim[n] - TK * t - 4 * g4;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (16 * h + i >= rel) s[n][h][i] = -INFINITY;
+            float mx = fmaxf(fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][0][2], s[n][0][3])),
+                             fmaxf(fmaxf(s[n][1][0], s[n][1][1]), fmaxf(s[n][1][2], s[n][1][3])));
+            if (__builtin_amdgcn_ballot_w64(mx * c2 > thr[n])) {
+                const float mt = max4(mx) * c2;
+                const bool move = mt > thr[n];
+                const float alpha = move ? __builtin_amdgcn_exp2f(m[n] - mt) : 1.f;  // 0 while m was -inf
+                if (move) {
+                    m[n] = mt;
+                    thr[n] = mt + kLazy;
+                    neg_m[n] = -mt;
+                }
+                lsum[n] *= alpha;
+#pragma unroll
+                for (int d = 0; d < DB; ++d) o[n][d] *= alpha;
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][h][i], c2, neg_m[n]));
+                    lsum[n] += e;
+                    pf[n][4 * h + i] = static_cast<T>(e);
+                }
+        }
+        const T* vsrc = vl + (4 * g4 + (l16 >> 2)) * VP + 4 * (l16 & 3);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+            const u32x2 lo = tr_read(vsrc + 16 * d), hi = tr_read(vsrc + 16 * VP + 16 * d);
+            const v8 vf = __builtin_bit_cast(v8, u32x4{lo[0], lo[1], hi[0], hi[1]});
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) o[n][d] = Mfma16<T>::run(vf, pf[n], o[n][d]);
+        }
+    }
+
+    // The four wavefronts merge pairwise in LDS (the V tiles are done with): 2 and 3 hand their
+    // states to 0 and 1, then 1 to 0.
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) lsum[n] = sum4(lsum[n]);
+    float* const ex = reinterpret_cast<float*>(smem);
+    float* const st = ex + 2 * NQ * 16 * CP;
+#pragma unroll
+    for (int half = 2; half >= 1; half >>= 1) {
+        __syncthreads();
+        if (wave >= half && wave < 2 * half) {
+            const int slot = wave - half;
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+                    *reinterpret_cast<f32x4*>(ex + ((slot * NQ + n) * 16 + l16) * CP + 16 * d + 4 * g4) = o[n][d];
+                if (g4 == 0) *reinterpret_cast<f32x2*>(st + ((slot * NQ + n) * 16 + l16) * 2) = f32x2{m[n], lsum[n]};
+            }
+        }
+        __syncthreads();
+        if (wave < half) {
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                const f32x2 other = *reinterpret_cast<const f32x2*>(st + ((wave * NQ + n) * 16 + l16) * 2);
+                const float mn = fmaxf(m[n], other[0]);
+                const float wa = m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[n] - mn);
+                const float wb = other[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(other[0] - mn);
+                m[n] = mn;
+                lsum[n] = lsum[n] * wa + other[1] * wb;
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    const f32x4 x = *reinterpret_cast<const f32x4*>(ex + ((wave * NQ + n) * 16 + l16) * CP + 16 * d + 4 * g4);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[n][d][i] = o[n][d][i] * wa + x[i] * wb;
+                }
+            }
+        }
+    }
+    if (wave != 0) return;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        if (!valid[n]) continue;
+        const float inv = lsum[n] > 0.f ? 1.f / lsum[n] : 0.f;
+        const int64_t tok = sp.q0 + pos[n];
+        if (alone) {
+            T* dst = static_cast<T*>(p.out) + head[n] * p.os[1] + tok * p.os[2];
+            typedef T t4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                const int col = 16 * d + 4 * g4;
+                if (col >= p.dv) continue;
+                t4 w;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = from_f32<T>(o[n][d][i] * inv);
+                *reinterpret_cast<t4*>(dst + col) = w;
+            }
+            if (p.lse && g4 == 0)
+                p.lse[head[n] * p.ls[1] + tok * p.ls[2]] = lsum[n] > 0.f ? (m[n] + log2f(lsum[n])) * kLn2f : -INFINITY;
+        } else {
+            const int64_t at = (static_cast<int64_t>(split) * p.rows_total + tok) * p.hq + head[n];
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                const int col = 16 * d + 4 * g4;
+                if (col < p.dv) *reinterpret_cast<f32x4*>(p.part_o + at * DP + col) = o[n][d] * inv;
+            }
+            if (g4 == 0) p.part_lse[at] = lsum[n] > 0.f ? m[n] + log2f(lsum[n]) : -INFINITY;
+        }
+    }
+}
+
+template <typename T, int DP, int NQ, bool FOUR>
+hipError_t launch_decode_as(const AttnParams& p, hipStream_t stream) {
+    constexpr size_t lds = decode_lds<T, DP, NQ>();
+    if constexpr (lds > 64 * 1024) {
+        static const hipError_t attr =
+            hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_decode_kernel<T, DP, NQ, FOUR>),
+                                hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
+        if (attr != hipSuccess) return attr;
+    }
+    hipLaunchKernelGGL((paged_decode_kernel<T, DP, NQ, FOUR>),
+                       dim3(static_cast<unsigned>(p.batch * p.hkv * p.splits + 1)), dim3(THREADS), lds, stream, p);
+    return hipGetLastError();
+}
+
+template <typename T, int DP>
+hipError_t launch_decode(const AttnParams& p, int rows, bool four, hipStream_t stream) {
+    if (four) return rows == 16 ? launch_decode_as<T, DP, 1, true>(p, stream) : launch_decode_as<T, DP, 2, true>(p, stream);
+    return rows == 16 ? launch_decode_as<T, DP, 1, false>(p, stream) : launch_decode_as<T, DP, 2, false>(p, stream);
+}
+
+}  // namespace paged
+}  // namespace kmi

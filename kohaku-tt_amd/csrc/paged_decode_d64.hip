@@ -1,0 +1,9 @@
+// Attention over a paged cache, padded head dim 64 (kernels in paged_decode.hpp).
+#include "paged_decode.hpp"
+
+namespace kmi {
+namespace paged {
+template hipError_t launch_decode<bf16, 64>(const AttnParams&, int, bool, hipStream_t);
+template hipError_t launch_decode<f16, 64>(const AttnParams&, int, bool, hipStream_t);
+}  // namespace paged
+}  // namespace kmi

@@ -15,7 +15,9 @@ PrivateUse1 when ``kohakutt`` is imported, ``src/kohakutt/torch_backend/registra
   build's ``_sdpa_varlen_offsets`` (tensor offsets, per-row packed masks), all
   differentiable where the reference's are;
 * ``torch.nn.attention.varlen.varlen_attn`` (``torch_attn::_varlen_attn`` and its
-  backward) on GPU tensors.
+  backward) on GPU tensors;
+* rotary positions and a paged key / value cache in 16 or 4 bits with the attention that
+  reads it (``rotary``, ``paged_append``, ``paged_read``, ``sdpa_paged``; ``paged.py``).
 
 Calls the kernels do not take keep torch's own CUDA/HIP paths.  The package raises
 ImportError when its native libraries are missing: there is no CPU or eager fallback.
@@ -47,9 +49,19 @@ _load()
 
 from . import attention  # noqa: E402
 from . import chains  # noqa: E402,F401
+from . import paged  # noqa: E402
 from .attention import sdpa, sdpa_varlen  # noqa: E402,F401
+from .paged import (  # noqa: E402,F401
+    paged_append,
+    paged_cache,
+    paged_read,
+    rotary,
+    rotary_frequencies,
+    sdpa_paged,
+)
 
 attention.install()
+paged.install()
 
 AVAILABLE = True
 

@@ -2,7 +2,8 @@
 
 * ``libkohakutt_amd.so`` -- the HIP kernels and the C ABI (``include/kohakutt_amd.h``),
   built with ``hipcc --offload-arch=gfx950``; no torch.
-* ``_torch_ops.so`` -- the torch op registrations (``csrc/torch_ops.cpp``), a host-only
+* ``_torch_ops.so`` -- the torch op registrations (``csrc/torch_ops.cpp``,
+  ``csrc/torch_paged.cpp``), a host-only
   C++ library linked against torch and ``libkohakutt_amd.so`` and loaded with
   ``torch.ops.load_library``.
 
@@ -40,6 +41,11 @@ HIP_SOURCES = [
     "attention_pipe.hip",
     "attention_bwd.hip",
     *[f"attention_bwd_d{d}.hip" for d in (32, 64, 96, 128)],
+    "rotary.hip",
+    "paged_cache.hip",
+    "paged_attention.hip",
+    *[f"paged_decode_d{d}.hip" for d in (32, 64, 96, 128, 192, 256)],
+    *[f"paged_tile_d{d}.hip" for d in (32, 64, 96, 128, 192, 256)],
 ]
 HIP_FLAGS = [
     f"--offload-arch={ARCH}",
@@ -74,13 +80,16 @@ def _run(cmd):
 # max needs no NaN canonicalisation there.
 SOURCE_FLAGS = {f"attention_d{d}.hip": ["-fno-honor-nans"] for d in (32, 64, 96, 128, 192, 256, "_pipe")}
 SOURCE_FLAGS.update({f"attention_tile_d{d}.hip": ["-fno-honor-nans"] for d in (32, 64, 96, 128, 192, 256)})
+SOURCE_FLAGS.update({f"paged_tile_d{d}.hip": ["-fno-honor-nans"] for d in (32, 64, 96, 128, 192, 256)})
 # The unit holding the DMA-staged forward kernels also prints the compiler's per-kernel
 # resource usage, which check_dma_spills reads.
 RESOURCE_REMARKS = "-Rpass-analysis=kernel-resource-usage"
 SOURCE_FLAGS["attention_d64.hip"] = SOURCE_FLAGS["attention_d64.hip"] + [RESOURCE_REMARKS]
 # So do the units of the 32x32x16 tile kernels, for check_tile_spills.
 TILE_SOURCES = [src for src in HIP_SOURCES if re.fullmatch(r"attention_(tile|bwd)_d\d+\.hip", src)]
-for _src in TILE_SOURCES:
+# (The same kernels over a paged cache.)
+PAGED_TILE_SOURCES = [src for src in HIP_SOURCES if re.fullmatch(r"paged_tile_d\d+\.hip", src)]
+for _src in TILE_SOURCES + PAGED_TILE_SOURCES:
     SOURCE_FLAGS[_src] = SOURCE_FLAGS.get(_src, []) + [RESOURCE_REMARKS]
 # The most vector registers a tile kernel may spill (14 today, masked backward at head dim 64).
 # Their waits count no loads, so a spill is slow, not wrong: 1x24x4396x128 backward with its
@@ -158,7 +167,7 @@ def build_capi(jobs: int = 8) -> Path:
     with concurrent.futures.ThreadPoolExecutor(max_workers=jobs) as pool:
         outs = list(pool.map(_run, cmds))
     for src, out in zip(HIP_SOURCES, outs):
-        if src in TILE_SOURCES:
+        if src in TILE_SOURCES + PAGED_TILE_SOURCES:
             if check_tile_spills(out) == 0:
                 raise RuntimeError(f"{src}: no tile kernel in the resource remarks")
         elif RESOURCE_REMARKS in SOURCE_FLAGS.get(src, []) and check_dma_spills(out) == 0:
@@ -179,13 +188,16 @@ def _torch_paths():
     return incs, libdir, abi
 
 
+TORCH_SOURCES = ["torch_ops.cpp", "torch_paged.cpp"]
+
+
 def build_torch_ops() -> Path:
-    """Compiles ``csrc/torch_ops.cpp`` into ``_torch_ops.so``."""
+    """Compiles the torch op registrations into ``_torch_ops.so``."""
     incs, libdir, abi = _torch_paths()
     BUILD.mkdir(exist_ok=True)
-    obj = BUILD / "torch_ops.o"
     cxx = os.environ.get("CXX", "g++")
-    _run(
+    objs = [BUILD / (Path(src).stem + ".o") for src in TORCH_SOURCES]
+    cmds = [
         [
             cxx,
             "-O2",
@@ -200,18 +212,21 @@ def build_torch_ops() -> Path:
             f"-I{ROCM / 'include'}",
             f"-I{INCLUDE}",
             "-c",
-            str(CSRC / "torch_ops.cpp"),
+            str(CSRC / src),
             "-o",
             str(obj),
         ]
-    )
+        for src, obj in zip(TORCH_SOURCES, objs)
+    ]
+    with concurrent.futures.ThreadPoolExecutor(max_workers=len(cmds)) as pool:
+        list(pool.map(_run, cmds))
     tmp = OPS_LIB.with_suffix(".so.tmp")
     _run(
         [
             cxx,
             "-shared",
             "-fPIC",
-            str(obj),
+            *map(str, objs),
             "-o",
             str(tmp),
             f"-L{PKG}",

@@ -32,6 +32,12 @@ EXPORTS = (
     "kmi_rms_norm_bwd",
     "kmi_layer_norm_bwd_workspace_bytes",
     "kmi_layer_norm_bwd",
+    "kmi_rotary",
+    "kmi_paged_append",
+    "kmi_paged_read",
+    "kmi_paged_attn_workspace_bytes",
+    "kmi_paged_attn_kernel",
+    "kmi_paged_attn",
     "kmi_last_error",
     "kmi_abi_version",
 )
@@ -125,6 +131,102 @@ class AttnBwdArgs(ctypes.Structure):
     ]
 
 
+_I64x2 = ctypes.c_int64 * 2
+
+
+class RotaryArgs(ctypes.Structure):
+    """``kmi_rotary_args``, field for field."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p * 2),
+        ("y", ctypes.c_void_p * 2),
+        ("heads", _I64x2),
+        ("x_stride", _I64x3 * 2),
+        ("y_stride", _I64x3 * 2),
+        ("dtype", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("inverse", ctypes.c_int32),
+        ("position_bits", ctypes.c_int32),
+        ("batch", ctypes.c_int64),
+        ("seq", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("rotary_dim", ctypes.c_int64),
+        ("positions", ctypes.c_void_p),
+        ("position_stride", _I64x2),
+        ("inv_freq", ctypes.c_void_p),
+        ("scale", ctypes.c_double),
+    ]
+
+
+class PagedCache(ctypes.Structure):
+    """``kmi_paged_cache``, field for field."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("k_stride", _I64x3),
+        ("v_stride", _I64x3),
+        ("k_scale_stride", _I64x3),
+        ("v_scale_stride", _I64x3),
+        ("dtype", ctypes.c_int32),
+        ("bits", ctypes.c_int32),
+        ("pages", ctypes.c_int64),
+        ("page_size", ctypes.c_int64),
+        ("heads_kv", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("head_dim_v", ctypes.c_int64),
+        ("block_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("table_width", ctypes.c_int64),
+        ("key_lengths", ctypes.c_void_p),
+        ("cu_seqlens", ctypes.c_void_p),
+        ("batch", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+    ]
+
+
+class PagedAppendArgs(ctypes.Structure):
+    """``kmi_paged_append_args``, field for field."""
+
+    _fields_ = [
+        ("cache", PagedCache),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("q", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p),
+        ("k_stride", _I64x2),
+        ("v_stride", _I64x2),
+        ("q_stride", _I64x2),
+        ("q_out_stride", _I64x2),
+        ("heads_q", ctypes.c_int64),
+        ("inv_freq", ctypes.c_void_p),
+        ("rotary_dim", ctypes.c_int64),
+        ("interleaved", ctypes.c_int32),
+        ("rotary_scale", ctypes.c_double),
+    ]
+
+
+class PagedAttnArgs(ctypes.Structure):
+    """``kmi_paged_attn_args``, field for field."""
+
+    _fields_ = [
+        ("cache", PagedCache),
+        ("q", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("q_stride", _I64x2),
+        ("o_stride", _I64x2),
+        ("lse_stride", _I64x2),
+        ("heads_q", ctypes.c_int64),
+        ("max_q", ctypes.c_int64),
+        ("max_k", ctypes.c_int64),
+        ("causal", ctypes.c_int32),
+        ("scale", ctypes.c_double),
+    ]
+
+
 class KmiError(RuntimeError):
     def __init__(self, status, message):
         super().__init__(f"kmi status {status}: {message}")
@@ -157,6 +259,12 @@ def lib():
         h.kmi_layer_norm_bwd_workspace_bytes.argtypes = [i64, i64, ctypes.POINTER(ctypes.c_size_t)]
         h.kmi_layer_norm_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i32, i32, i32, vp,
                                          ctypes.c_size_t, vp]
+        h.kmi_rotary.argtypes = [ctypes.POINTER(RotaryArgs), vp]
+        h.kmi_paged_append.argtypes = [ctypes.POINTER(PagedAppendArgs), vp]
+        h.kmi_paged_read.argtypes = [ctypes.POINTER(PagedCache), vp, vp, i64, vp]
+        h.kmi_paged_attn_workspace_bytes.argtypes = [ctypes.POINTER(PagedAttnArgs), ctypes.POINTER(ctypes.c_size_t)]
+        h.kmi_paged_attn_kernel.argtypes = [ctypes.POINTER(PagedAttnArgs), ctypes.POINTER(ctypes.c_char_p)]
+        h.kmi_paged_attn.argtypes = [ctypes.POINTER(PagedAttnArgs), vp, ctypes.c_size_t, vp]
         h.kmi_last_error.restype = ctypes.c_char_p
         h.kmi_last_error.argtypes = []
         h.kmi_abi_version.argtypes = []
@@ -199,3 +307,32 @@ def layer_norm_fwd(x, w, b, y, mean, rstd, rows, width, x_dtype, w_dtype, b_dtyp
 
 def rms_norm_fwd(x, w, b, y, rstd, rows, width, x_dtype, w_dtype, b_dtype, eps, stream) -> None:
     check(lib().kmi_rms_norm_fwd(x, w, b, y, rstd, rows, width, x_dtype, w_dtype, b_dtype, eps, stream))
+
+
+def rotary(args: RotaryArgs, stream: int) -> None:
+    check(lib().kmi_rotary(ctypes.byref(args), stream))
+
+
+def paged_append(args: PagedAppendArgs, stream: int) -> None:
+    check(lib().kmi_paged_append(ctypes.byref(args), stream))
+
+
+def paged_read(cache: PagedCache, k_out: int, v_out: int, max_k: int, stream: int) -> None:
+    check(lib().kmi_paged_read(ctypes.byref(cache), k_out, v_out, max_k, stream))
+
+
+def paged_attn_workspace_bytes(args: PagedAttnArgs) -> int:
+    n = ctypes.c_size_t(0)
+    check(lib().kmi_paged_attn_workspace_bytes(ctypes.byref(args), ctypes.byref(n)))
+    return n.value
+
+
+def paged_attn_kernel(args: PagedAttnArgs) -> str:
+    """The kernel ``kmi_paged_attn`` runs the call on."""
+    name = ctypes.c_char_p()
+    check(lib().kmi_paged_attn_kernel(ctypes.byref(args), ctypes.byref(name)))
+    return name.value.decode()
+
+
+def paged_attn(args: PagedAttnArgs, workspace: int, workspace_bytes_: int, stream: int) -> None:
+    check(lib().kmi_paged_attn(ctypes.byref(args), workspace, workspace_bytes_, stream))
