@@ -105,6 +105,13 @@ __device__ __forceinline__ void turn(double pos, float freq, double& c, double& 
     sincospi(r + r, &s, &c);
 }
 
+// A pair turned, with its products and sums in one order everywhere (left to the compiler, which
+// of the two products is fused differs from kernel to kernel).
+__device__ __forceinline__ void turned(float x1, float x2, float c, float s, float& y1, float& y2) {
+    y1 = __builtin_fmaf(x1, c, -(x2 * s));
+    y2 = __builtin_fmaf(x2, c, x1 * s);
+}
+
 // ---------------------------------------------------------------- 4 bits
 
 // Two of the values a dword of eight codes stands for (codes 2 sel and 2 sel + 1) times the

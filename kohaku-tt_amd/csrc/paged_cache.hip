@@ -1,13 +1,17 @@
 // The paged cache: its host checks, kmi_paged_append and kmi_paged_read.
 //
-// Append: a thread owns a chunk of dims of one token, turns its share of the token's query
-// and key heads with sines and cosines formed once, and copies or quantises values.  16-bit
-// rows move as 16-byte vectors (bound by memory); a 4-bit row's groups of 32 dims lie in four
-// neighbouring lanes, eight dims each, which agree on the group's exponent by two lane
-// exchanges.  Rotated keys are formed in 64 bits there: a value that 32 bits put on the wrong
-// side of a border between two codes would come out a whole step off.
+// Append: a workgroup owns a few tokens.  Its threads request their vectors of queries, keys and
+// values, find the tokens' places (one thread a token) and form their sines and cosines into LDS
+// behind those loads' latency, and then turn, quantise and store, so that nothing waits for a
+// token's chain of lengths, table entry and angle but the stores.  16-bit rows move as 16-byte
+// vectors (bound by memory); a 4-bit row's groups of 32 dims lie in four neighbouring lanes,
+// eight dims each, which agree on the group's exponent by two lane exchanges.  Rotated keys are
+// formed in 64 bits there: a value that 32 bits put on the wrong side of a border between two
+// codes would come out a whole step off.
 //
-// Read: one 16-byte store per thread, its row found through the table.
+// Read: four 16-byte stores a thread, their rows found through the table.
+#include <algorithm>
+
 #include "paged.hpp"
 
 namespace kmi {
@@ -83,7 +87,9 @@ Cache device_cache(const kmi_paged_cache& c) {
 namespace {
 
 constexpr int THREADS = 256;
-constexpr int MOST = 512;  // threads of an append whose token needs more than 256
+constexpr int ITEMS = 4;    // of a thread, in flight together
+constexpr int TOKENS = 64;  // of a workgroup, at most
+constexpr int PAIRS = 1024; // angles of a workgroup, at most
 
 struct AppendParams {
     Cache c;
@@ -95,10 +101,94 @@ struct AppendParams {
     int hq, rd, inter;
     const float* freq;
     double scale;
-    int hg, nk, nv;  // threads that share a chunk's heads; chunks of a key (query) row, of a value row
-    int tpt, tpb;
-    fwd::FastDiv fd_tpt, fd_chunks;
+    int nk, nv;    // chunks of a query or key row, of a value row
+    // Workgroups of queries and keys come first, those of values behind them: items (vectors, or
+    // pairs of them) of a token and tokens of a workgroup for each.
+    int per_qk, per_v, tpb_qk, tpb_v, blocks_qk;
+    fwd::FastDiv fd_qk, fd_v, fd_nk, fd_nv, fd_half;
 };
+
+// A token's page (-1: none), row there and position (-1: none).
+struct Held {
+    int page, row, pos, pad;
+};
+
+// The places of a workgroup's tokens and, for rotated calls, their angles' cosines and sines (F:
+// float or double), into LDS.  Tokens of one sequence (nearly every workgroup's) find it by scalar
+// loads, which do not queue behind the vectors in flight, and wait for one vector load, the
+// table's; a workgroup across sequences searches per token.
+template <typename F>
+__device__ __forceinline__ void place_tokens(const AppendParams& p, int t0, int nt, Held* held, F* cosine, F* sine) {
+    const Cache& c = p.c;
+    const int half = cosine ? p.rd / 2 : 0;
+    int seq = t0, first = 0, lq = 1;
+    bool one = nt == 1;
+    if (c.cu) {
+        int lo = 0, hi = c.batch;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (uniform_i32(c.cu + mid) <= t0)
+                lo = mid;
+            else
+                hi = mid - 1;
+        }
+        seq = min(lo, max(c.batch - 1, 0));
+        const int start = uniform_i32(c.cu + seq), end = uniform_i32(c.cu + min(seq + 1, c.batch));
+        one = start >= 0 && start <= t0 && t0 + nt <= end && end <= c.tokens;
+        first = t0 - start;
+        lq = end - start;
+    }
+    int64_t pos0 = 0;
+    if (one) pos0 = static_cast<int64_t>(uniform_i32(c.klen + seq)) - lq + first;
+    if (static_cast<int>(threadIdx.x) < nt) {
+        Place at{seq, -1};
+        if (!one)
+            at = place_of(c, t0 + threadIdx.x);
+        else if (pos0 + threadIdx.x >= 0 && pos0 + threadIdx.x < c.capacity)
+            at.pos = static_cast<int>(pos0 + threadIdx.x);
+        Held h{-1, 0, at.pos, 0};
+        if (at.pos >= 0) h.page = page_of(c, at.seq, at.pos, h.row);
+        held[threadIdx.x] = h;
+    }
+    if (!one) __syncthreads();  // (uniform)
+    for (int i = threadIdx.x; i < nt * half; i += THREADS) {
+        const int tl = fwd::fdiv(i, p.fd_half);
+        const double pos = one ? static_cast<double>(pos0 + tl) : static_cast<double>(held[tl].pos);
+        F cs, sn;
+        turn(pos, p.freq[i - tl * half], cs, sn);
+        cosine[i] = cs * static_cast<F>(p.scale);
+        sine[i] = sn * static_cast<F>(p.scale);
+    }
+    __syncthreads();
+}
+
+// An item of a workgroup: its token, head and chunk.  Query heads come before key heads.
+struct Item {
+    int tl, h, c;
+};
+__device__ __forceinline__ Item item_of(int i, int per, fwd::FastDiv fd_per, int chunks, fwd::FastDiv fd_chunks) {
+    Item m;
+    m.tl = fwd::fdiv(i, fd_per);
+    const int r = i - m.tl * per;
+    m.h = fwd::fdiv(r, fd_chunks);
+    m.c = r - m.h * chunks;
+    return m;
+}
+__device__ __forceinline__ Item qk_item(const AppendParams& p, int i) { return item_of(i, p.per_qk, p.fd_qk, p.nk, p.fd_nk); }
+__device__ __forceinline__ Item v_item(const AppendParams& p, int i) { return item_of(i, p.per_v, p.fd_v, p.nv, p.fd_nv); }
+
+// The source row of a query or key head, and the place of a cache row (codes, or 16-bit values).
+template <typename T>
+__device__ __forceinline__ const T* qk_row(const AppendParams& p, int64_t t, int h) {
+    return h < p.hq ? static_cast<const T*>(p.q) + t * p.qs[0] + h * p.qs[1]
+                    : static_cast<const T*>(p.k) + t * p.ks[0] + (h - p.hq) * p.ks[1];
+}
+__device__ __forceinline__ char* k_place(const AppendParams& p, const Held& at, int h) {
+    return p.c.k + at.page * p.c.ks[0] + h * p.c.ks[1] + at.row * p.c.ks[2];
+}
+__device__ __forceinline__ char* v_place(const AppendParams& p, const Held& at, int h) {
+    return p.c.v + at.page * p.c.vs[0] + h * p.c.vs[1] + at.row * p.c.vs[2];
+}
 
 template <typename T>
 struct Vec8;
@@ -115,85 +205,122 @@ using V8 = typename Vec8<T>::type;
 
 // ---------------------------------------------------------------- 16 bits
 
-// Key chunks of VW dims a half (both vectors of a rotated pair in one thread), value chunks of
-// eight dims.  VW is 8, or 1 where the rotated dims are no whole pairs of vectors.
-template <typename T, int VW>
-__global__ __launch_bounds__(MOST) void append_kernel(const AppendParams p) {
-    const int tl = fwd::fdiv(threadIdx.x, p.fd_tpt);
-    const int t = blockIdx.x * p.tpb + tl;
-    if (tl >= p.tpb || t >= p.c.tokens) return;
-    const int rem = threadIdx.x - tl * p.tpt;
-    const int hg = fwd::fdiv(rem, p.fd_chunks);
-    int c = rem - hg * (p.nk + p.nv);
-    const Place at = place_of(p.c, t);
-    int row = 0;
-    const int page = at.pos >= 0 ? page_of(p.c, at.seq, at.pos, row) : -1;
-    if (c >= p.nk) {
-        c -= p.nk;
-        if (page < 0) return;
-        for (int h = hg; h < p.c.hkv; h += p.hg) {
-            const u32x4 x = *reinterpret_cast<const u32x4*>(static_cast<const T*>(p.v) + t * p.vs[0] + h * p.vs[1] + 8 * c);
-            *reinterpret_cast<u32x4*>(p.c.v + page * p.c.vs[0] + h * p.c.vs[1] + row * p.c.vs[2] + 16 * c) = x;
+// A workgroup of values: `out` stores a chunk of eight dims at its place.
+template <typename T, typename F>
+__device__ __forceinline__ void append_values(const AppendParams& p, int block, Held* held, F out) {
+    const int t0 = block * p.tpb_v;
+    const int nt = min(p.tpb_v, p.c.tokens - t0);
+    const int items = nt * p.per_v;
+    for (int base = 0; base < items; base += ITEMS * THREADS) {
+        V8<T> x[ITEMS];
+#pragma unroll
+        for (int j = 0; j < ITEMS; ++j) {
+            const int i = base + j * THREADS + threadIdx.x;
+            if (i >= items) continue;
+            const Item m = v_item(p, i);
+            x[j] = *reinterpret_cast<const V8<T>*>(static_cast<const T*>(p.v) + static_cast<int64_t>(t0 + m.tl) * p.vs[0] +
+                                                   m.h * p.vs[1] + 8 * m.c);
         }
+        if (base == 0) place_tokens<float>(p, t0, nt, held, nullptr, nullptr);
+#pragma unroll
+        for (int j = 0; j < ITEMS; ++j) {
+            const int i = base + j * THREADS + threadIdx.x;
+            if (i >= items) break;
+            const Item m = v_item(p, i);
+            const Held at = held[m.tl];
+            if (at.page >= 0) out(at, m.h, m.c, x[j]);
+        }
+    }
+}
+
+// Query and key chunks of VW dims a half: both vectors of a rotated pair in one thread.  VW is 8,
+// or 1 where the rotated dims are no whole pairs of vectors.
+template <typename T, int VW, bool INTER>
+__global__ __launch_bounds__(THREADS) void append_kernel(const AppendParams p) {
+    __shared__ __align__(16) float cosine[PAIRS], sine[PAIRS];
+    __shared__ Held held[TOKENS];
+    if (static_cast<int>(blockIdx.x) >= p.blocks_qk) {
+        append_values<T>(p, blockIdx.x - p.blocks_qk, held, [&](const Held& at, int h, int c, const V8<T>& x) {
+            *reinterpret_cast<V8<T>*>(v_place(p, at, h) + 16 * c) = x;
+        });
         return;
     }
-    const int nrot = p.rd / (2 * VW);
-    const bool rot = c < nrot;
-    const int lo = rot ? (p.inter ? 2 * VW * c : VW * c) : p.rd + VW * (c - nrot);
-    const int hi = rot ? (p.inter ? lo + VW : lo + p.rd / 2) : lo;
-    float cs[VW], sn[VW];
-    if (rot) {
+    const int t0 = blockIdx.x * p.tpb_qk;
+    const int nt = min(p.tpb_qk, p.c.tokens - t0);
+    const int items = nt * p.per_qk;
+    const int half = p.rd / 2, nrot = half / VW;
+    struct Vec {
+        T e[VW];
+    };
+    auto first_dim = [&](int c) { return c < nrot ? (INTER ? 2 * VW * c : VW * c) : p.rd + VW * (c - nrot); };
+    auto load = [&](const T* from) {
+        Vec v;
+        __builtin_memcpy(&v, __builtin_assume_aligned(from, VW * 2), VW * 2);
+        return v;
+    };
+    auto store = [&](T* to, const Vec& v) { __builtin_memcpy(__builtin_assume_aligned(to, VW * 2), &v, VW * 2); };
+    const int apart = INTER ? VW : half;
+    Vec a[ITEMS], z[ITEMS];
+    auto fetch = [&](int base) {
 #pragma unroll
-        for (int i = 0; i < VW; ++i) {
-            turn(static_cast<double>(at.pos), p.freq[VW * c + i], cs[i], sn[i]);
-            cs[i] *= static_cast<float>(p.scale);
-            sn[i] *= static_cast<float>(p.scale);
+        for (int j = 0; j < ITEMS; ++j) {
+            const int i = base + j * THREADS + threadIdx.x;
+            if (i >= items) continue;
+            const Item m = qk_item(p, i);
+            const T* src = qk_row<T>(p, t0 + m.tl, m.h) + first_dim(m.c);
+            a[j] = load(src);
+            if (m.c < nrot) z[j] = load(src + apart);
         }
-    }
-    for (int h = hg; h < p.hq + p.c.hkv; h += p.hg) {
-        const bool query = h < p.hq;
-        const T* src;
-        T* dst;
-        if (query) {
-            src = static_cast<const T*>(p.q) + t * p.qs[0] + h * p.qs[1];
-            dst = static_cast<T*>(p.qo) + t * p.qos[0] + h * p.qos[1];
-        } else {
-            if (page < 0) return;
-            const int hk = h - p.hq;
-            src = static_cast<const T*>(p.k) + t * p.ks[0] + hk * p.ks[1];
-            dst = reinterpret_cast<T*>(p.c.k + page * p.c.ks[0] + hk * p.c.ks[1] + row * p.c.ks[2]);
-        }
-        T a[VW], z[VW];
-        __builtin_memcpy(a, __builtin_assume_aligned(src + lo, VW * 2), VW * 2);
-        __builtin_memcpy(z, __builtin_assume_aligned(src + hi, VW * 2), VW * 2);
-        T u[VW], w[VW];
-        if (query && at.pos < 0) {
-            // A row of no sequence (or past the cache).
+    };
+    fetch(0);
+    place_tokens(p, t0, nt, held, cosine, sine);
+    for (int base = 0;;) {
 #pragma unroll
-            for (int i = 0; i < VW; ++i) u[i] = w[i] = static_cast<T>(0.f);
-        } else if (!rot) {
-#pragma unroll
-            for (int i = 0; i < VW; ++i) u[i] = w[i] = a[i];
-        } else if (VW > 1 && p.inter) {
-#pragma unroll
-            for (int i = 0; i < VW; ++i) {
-                const T* in = i < VW / 2 ? a : z;
-                T* out = i < VW / 2 ? u : w;
-                const int e = VW > 1 ? 2 * (i % (VW / 2 > 0 ? VW / 2 : 1)) : 0;
-                const float x1 = to_f32(in[e]), x2 = to_f32(in[e + (VW > 1)]);
-                out[e] = from_f32<T>(x1 * cs[i] - x2 * sn[i]);
-                out[e + (VW > 1)] = from_f32<T>(x2 * cs[i] + x1 * sn[i]);
+        for (int j = 0; j < ITEMS; ++j) {
+            const int i = base + j * THREADS + threadIdx.x;
+            if (i >= items) break;
+            const Item m = qk_item(p, i);
+            const Held at = held[m.tl];
+            T* dst;
+            if (m.h < p.hq) {
+                dst = static_cast<T*>(p.qo) + static_cast<int64_t>(t0 + m.tl) * p.qos[0] + m.h * p.qos[1];
+                // A query of no sequence (or past the cache) is zero.
+                if (at.pos < 0) a[j] = z[j] = Vec{};
+            } else {
+                if (at.page < 0) continue;
+                dst = reinterpret_cast<T*>(k_place(p, at, m.h - p.hq));
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < VW; ++i) {
-                const float x1 = to_f32(a[i]), x2 = to_f32(z[i]);
-                u[i] = from_f32<T>(x1 * cs[i] - x2 * sn[i]);
-                w[i] = from_f32<T>(x2 * cs[i] + x1 * sn[i]);
+            dst += first_dim(m.c);
+            if (m.c >= nrot) {
+                store(dst, a[j]);
+                continue;
             }
+            float cs[VW], sn[VW];
+            __builtin_memcpy(cs, __builtin_assume_aligned(cosine + m.tl * half + VW * m.c, VW * 4), VW * 4);
+            __builtin_memcpy(sn, __builtin_assume_aligned(sine + m.tl * half + VW * m.c, VW * 4), VW * 4);
+            Vec u, w;
+            auto pair = [&](T p1, T p2, int e, T& y1, T& y2) {
+                float f1, f2;
+                turned(to_f32(p1), to_f32(p2), cs[e], sn[e], f1, f2);
+                y1 = from_f32<T>(f1);
+                y2 = from_f32<T>(f2);
+            };
+            if constexpr (INTER && VW > 1) {
+#pragma unroll
+                for (int e = 0; e < VW / 2; ++e) {
+                    pair(a[j].e[2 * e], a[j].e[2 * e + 1], e, u.e[2 * e], u.e[2 * e + 1]);
+                    pair(z[j].e[2 * e], z[j].e[2 * e + 1], VW / 2 + e, w.e[2 * e], w.e[2 * e + 1]);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < VW; ++e) pair(a[j].e[e], z[j].e[e], e, u.e[e], w.e[e]);
+            }
+            store(dst, u);
+            store(dst + apart, w);
         }
-        __builtin_memcpy(__builtin_assume_aligned(dst + lo, VW * 2), u, VW * 2);
-        if (rot) __builtin_memcpy(__builtin_assume_aligned(dst + hi, VW * 2), w, VW * 2);
+        base += ITEMS * THREADS;
+        if (base >= items) break;
+        fetch(base);
     }
 }
 
@@ -205,129 +332,157 @@ __device__ __forceinline__ int max_of_four(int v) {
     return max(v, __shfl_xor(v, 2, kWave));
 }
 
-// Eight values of a group of 32 (four neighbouring lanes hold it) as codes; `exponent`: the
-// group's scale byte.  The codes are those nearest to y 2^-e in exact arithmetic: the product
-// is exact in 64 bits and rounds to 32 toward zero with the last bit set where that drops
+// The group's scale byte and 2^-e from the largest exponent field (biased by `bias`, `top_field`
+// for infinities and NaN) of its values.
+struct Scale {
+    int byte, e;
+};
+__device__ __forceinline__ Scale group_scale(int field, int bias, int top_field) {
+    field = max_of_four(field);
+    const int e = field == 0 ? -127 : min(max(field - bias - 2, -126), 127);
+    return Scale{field == top_field ? 255 : e + 127, e};
+}
+
+// Eight values in units of the scale as codes: nearest, ties to even, saturating.
+__device__ __forceinline__ uint32_t codes_of(const float (&f)[8]) {
+    uint32_t codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, f[0], f[1], 1.f, 0);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, f[2], f[3], 1.f, 1);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, f[4], f[5], 1.f, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, f[6], f[7], 1.f, 3);
+}
+
+// Values of 16 bits: exact in 32 bits, and so is their product with a power of two (values that
+// vanish below 2^-149 are zeros in any code).
+template <typename T>
+__device__ __forceinline__ uint32_t quantise(const V8<T>& x, int& byte) {
+    float f[8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        f[i] = to_f32(x[i]);
+        top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
+    }
+    // (A subnormal bf16's exponent is below the smallest scale's, as a field of zero says; only
+    // zero itself keeps the byte 0.)
+    const int nonzero = max_of_four(top != 0);
+    Scale s = group_scale(static_cast<int>(top >> 23), 127, 255);
+    if (nonzero && s.byte == 0) s = Scale{1, -126};
+    byte = s.byte;
+    // 2^-e in two factors: e reaches 127.
+    const float a = __uint_as_float(static_cast<uint32_t>(127 - s.e / 2) << 23);
+    const float b = __uint_as_float(static_cast<uint32_t>(127 - (s.e - s.e / 2)) << 23);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = f[i] * a * b;
+    return codes_of(f);
+}
+
+// Rotated values in 64 bits: the codes are those nearest to y 2^-e in exact arithmetic.  The
+// product is exact in 64 bits and rounds to 32 toward zero with the last bit set where that drops
 // anything, which no border between two codes has (nearest rounding could land on one).
-__device__ __forceinline__ uint32_t quantise8(const double (&y)[8], int& exponent) {
+__device__ __forceinline__ uint32_t quantise(const double (&y)[8], int& byte) {
     int top = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = max(top, static_cast<int>(__double2hiint(y[i]) & 0x7fffffff));
-    top = max_of_four(top);
-    const int e64 = top >> 20;
-    const int e = e64 == 0 ? -127 : min(max(e64 - 1023 - 2, -126), 127);
-    exponent = e64 == 0x7ff ? 255 : e + 127;
-    const double inv = __hiloint2double((1023 - e) << 20, 0);
-    uint32_t codes = 0;
+    const Scale s = group_scale(top >> 20, 1023, 0x7ff);
+    byte = s.byte;
+    const double inv = __hiloint2double((1023 - s.e) << 20, 0);
     float f[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const double s = y[i] * inv;
-        f[i] = static_cast<float>(s);
+        const double x = y[i] * inv;
+        f[i] = static_cast<float>(x);
         const double back = static_cast<double>(f[i]);
-        if (back != s) {
+        if (back != x) {
             const uint32_t bits = __float_as_uint(f[i]);
-            f[i] = __uint_as_float((fabs(back) > fabs(s) ? bits - 1 : bits) | 1u);
+            f[i] = __uint_as_float((fabs(back) > fabs(x) ? bits - 1 : bits) | 1u);
         }
     }
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, f[0], f[1], 1.f, 0);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, f[2], f[3], 1.f, 1);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, f[4], f[5], 1.f, 2);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, f[6], f[7], 1.f, 3);
-    return codes;
+    return codes_of(f);
 }
 
 // Chunks of eight dims; head dims are whole groups, so a group's four chunks are four
-// neighbouring lanes that run the same heads.
-template <typename T>
+// neighbouring lanes with items of one token and head.
+template <typename T, bool INTER>
 __global__ __launch_bounds__(THREADS) void append4_kernel(const AppendParams p) {
-    const int tl = fwd::fdiv(threadIdx.x, p.fd_tpt);
-    const int t = blockIdx.x * p.tpb + tl;
-    if (tl >= p.tpb || t >= p.c.tokens) return;
-    const int rem = threadIdx.x - tl * p.tpt;
-    const int hg = fwd::fdiv(rem, p.fd_chunks);
-    int c = rem - hg * (p.nk + p.nv);
-    const Place at = place_of(p.c, t);
-    int row = 0;
-    const int page = at.pos >= 0 ? page_of(p.c, at.seq, at.pos, row) : -1;
+    __shared__ __align__(16) double cosine[PAIRS], sine[PAIRS];
+    __shared__ Held held[TOKENS];
     typedef V8<T> v8;
-    double y[8];
-    int exponent;
-    if (c >= p.nk) {
-        c -= p.nk;
-        if (page < 0) return;
-        for (int h = hg; h < p.c.hkv; h += p.hg) {
-            const v8 x = *reinterpret_cast<const v8*>(static_cast<const T*>(p.v) + t * p.vs[0] + h * p.vs[1] + 8 * c);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = static_cast<double>(to_f32(x[i]));
-            const uint32_t codes = quantise8(y, exponent);
-            *reinterpret_cast<uint32_t*>(p.c.v + page * p.c.vs[0] + h * p.c.vs[1] + row * p.c.vs[2] + 4 * c) = codes;
+    if (static_cast<int>(blockIdx.x) >= p.blocks_qk) {
+        append_values<T>(p, blockIdx.x - p.blocks_qk, held, [&](const Held& at, int h, int c, const v8& x) {
+            int byte;
+            *reinterpret_cast<uint32_t*>(v_place(p, at, h) + 4 * c) = quantise<T>(x, byte);
             if ((c & 3) == 0)
-                p.c.vsc[page * p.c.vss[0] + h * p.c.vss[1] + row * p.c.vss[2] + (c >> 2)] = static_cast<uint8_t>(exponent);
-        }
+                p.c.vsc[at.page * p.c.vss[0] + h * p.c.vss[1] + at.row * p.c.vss[2] + (c >> 2)] = static_cast<uint8_t>(byte);
+        });
         return;
     }
-    // Dim d = 8 c + i: its value times cs[i] plus its partner's times sn[i].
-    const int half = p.rd / 2, d0 = 8 * c;
-    double cs[8], sn[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int d = d0 + i;
-        cs[i] = 1.0;
-        sn[i] = 0.0;
-        if (d < p.rd) {
-            const bool first = p.inter ? (d & 1) == 0 : d < half;
-            // (An interleaved pair's angle is formed once.)
-            if (p.inter && !first && i > 0) {
-                cs[i] = cs[i - 1];
-                sn[i] = -sn[i - 1];
-                continue;
-            }
-            turn(static_cast<double>(at.pos), p.freq[p.inter ? d >> 1 : (first ? d : d - half)], cs[i], sn[i]);
-            cs[i] *= p.scale;
-            sn[i] *= first ? -p.scale : p.scale;
-        }
-    }
+    const int t0 = blockIdx.x * p.tpb_qk;
+    const int nt = min(p.tpb_qk, p.c.tokens - t0);
+    const int items = nt * p.per_qk;
+    const int half = p.rd / 2;
     // Half layout: whole partner vectors where a half is a number of chunks.
     const bool whole = half % 8 == 0;
-    for (int h = hg; h < p.hq + p.c.hkv; h += p.hg) {
-        const bool query = h < p.hq;
-        if (!query && page < 0) return;
-        const T* src = query ? static_cast<const T*>(p.q) + t * p.qs[0] + h * p.qs[1]
-                             : static_cast<const T*>(p.k) + t * p.ks[0] + (h - p.hq) * p.ks[1];
-        const v8 x = *reinterpret_cast<const v8*>(src + d0);
-        v8 z = x;
-        if (p.inter) {
+    v8 x[ITEMS], z[ITEMS];
+    auto fetch = [&](int base) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) z[i] = x[i ^ 1];
-        } else if (d0 < p.rd) {
+        for (int j = 0; j < ITEMS; ++j) {
+            const int i = base + j * THREADS + threadIdx.x;
+            if (i >= items) continue;
+            const Item m = qk_item(p, i);
+            const T* src = qk_row<T>(p, t0 + m.tl, m.h);
+            const int d0 = 8 * m.c;
+            x[j] = *reinterpret_cast<const v8*>(src + d0);
+            if (INTER || d0 >= p.rd) continue;
             if (whole) {
-                z = *reinterpret_cast<const v8*>(src + (d0 < half ? d0 + half : d0 - half));
+                z[j] = *reinterpret_cast<const v8*>(src + (d0 < half ? d0 + half : d0 - half));
             } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int d = d0 + i;
-                    if (d < p.rd) z[i] = src[d < half ? d + half : d - half];
+                for (int e = 0; e < 8; ++e) {
+                    const int d = d0 + e;
+                    z[j][e] = d < p.rd ? src[d < half ? d + half : d - half] : x[j][e];
                 }
             }
         }
+    };
+    fetch(0);
+    place_tokens(p, t0, nt, held, cosine, sine);
+    for (int base = 0;;) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const double own = static_cast<double>(to_f32(x[i]));
-            y[i] = d0 + i < p.rd ? own * cs[i] + static_cast<double>(to_f32(z[i])) * sn[i] : own;
-        }
-        if (query) {
-            v8 w;
+        for (int j = 0; j < ITEMS; ++j) {
+            const int i = base + j * THREADS + threadIdx.x;
+            if (i >= items) break;
+            const Item m = qk_item(p, i);
+            const Held at = held[m.tl];
+            if (m.h >= p.hq && at.page < 0) continue;  // (all four lanes of a group)
+            const int d0 = 8 * m.c;
+            double y[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = from_f32<T>(at.pos < 0 ? 0.f : static_cast<float>(y[i]));
-            *reinterpret_cast<v8*>(static_cast<T*>(p.qo) + t * p.qos[0] + h * p.qos[1] + d0) = w;
-        } else {
-            const uint32_t codes = quantise8(y, exponent);
-            const int hk = h - p.hq;
-            *reinterpret_cast<uint32_t*>(p.c.k + page * p.c.ks[0] + hk * p.c.ks[1] + row * p.c.ks[2] + 4 * c) = codes;
-            if ((c & 3) == 0)
-                p.c.ksc[page * p.c.kss[0] + hk * p.c.kss[1] + row * p.c.kss[2] + (c >> 2)] = static_cast<uint8_t>(exponent);
+            for (int e = 0; e < 8; ++e) {
+                const int d = d0 + e;
+                y[e] = static_cast<double>(to_f32(x[j][e]));
+                if (d >= p.rd) continue;
+                // Its value times the cosine plus or minus its partner's times the sine.
+                const bool first = INTER ? (e & 1) == 0 : d < half;
+                const int k = m.tl * half + (INTER ? d >> 1 : (first ? d : d - half));
+                const double other = static_cast<double>(to_f32(INTER ? x[j][e ^ 1] : z[j][e]));
+                y[e] = y[e] * cosine[k] + other * (first ? -sine[k] : sine[k]);
+            }
+            if (m.h < p.hq) {
+                v8 w;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] = from_f32<T>(at.pos < 0 ? 0.f : static_cast<float>(y[e]));
+                *reinterpret_cast<v8*>(static_cast<T*>(p.qo) + static_cast<int64_t>(t0 + m.tl) * p.qos[0] + m.h * p.qos[1] + d0) = w;
+                continue;
+            }
+            int byte;
+            const int h = m.h - p.hq;
+            *reinterpret_cast<uint32_t*>(k_place(p, at, h) + 4 * m.c) = quantise(y, byte);
+            if ((m.c & 3) == 0)
+                p.c.ksc[at.page * p.c.kss[0] + h * p.c.kss[1] + at.row * p.c.kss[2] + (m.c >> 2)] = static_cast<uint8_t>(byte);
         }
+        base += ITEMS * THREADS;
+        if (base >= items) break;
+        fetch(base);
     }
 }
 
@@ -377,22 +532,28 @@ hipError_t launch_append(const kmi_paged_append_args* a, hipStream_t stream) {
     const int vw = four ? 8 : (p.rd % 16 == 0 ? 8 : 1);
     p.nk = four ? p.c.d / 8 : p.rd / (2 * vw) + (p.c.d - p.rd) / vw;
     p.nv = p.c.dv / 8;
-    // Threads of a token: as in kmi_rotary, more of them where tokens are few.
-    const int heads = p.hq + p.c.hkv, per = p.nk + p.nv;
-    p.hg = 1;
-    while (2 * p.hg * per <= THREADS && p.hg < heads && tokens * per * p.hg < (1 << 17)) p.hg *= 2;
-    p.tpt = p.hg * per;
-    const int threads = p.tpt <= THREADS ? THREADS : MOST;
-    p.tpb = threads / p.tpt;
-    p.fd_tpt = fwd::fast_div(static_cast<uint32_t>(p.tpt));
-    p.fd_chunks = fwd::fast_div(static_cast<uint32_t>(per));
-    const dim3 grid(static_cast<unsigned>(ceil_div(tokens, p.tpb)));
+    p.per_qk = (p.hq + p.c.hkv) * p.nk;
+    p.per_v = p.c.hkv * p.nv;
+    // Tokens of a workgroup: a batch of items a thread, unless few tokens leave CUs idle.
+    const auto tokens_of = [&](int per, int64_t most) {
+        return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({ITEMS * THREADS / per, most, tokens / 1024})));
+    };
+    p.tpb_qk = tokens_of(p.per_qk, p.rd > 0 ? std::min(TOKENS, PAIRS / (p.rd / 2)) : TOKENS);
+    p.tpb_v = tokens_of(p.per_v, TOKENS);
+    p.blocks_qk = static_cast<int>(ceil_div(tokens, p.tpb_qk));
+    p.fd_qk = fwd::fast_div(static_cast<uint32_t>(p.per_qk));
+    p.fd_v = fwd::fast_div(static_cast<uint32_t>(p.per_v));
+    p.fd_nk = fwd::fast_div(static_cast<uint32_t>(p.nk));
+    p.fd_nv = fwd::fast_div(static_cast<uint32_t>(p.nv));
+    p.fd_half = fwd::fast_div(static_cast<uint32_t>(p.rd / 2));
+    const dim3 grid(static_cast<unsigned>(p.blocks_qk + ceil_div(tokens, p.tpb_v)));
+    auto enqueue = [&](void (*kernel)(AppendParams)) { hipLaunchKernelGGL(kernel, grid, dim3(THREADS), 0, stream, p); };
     if (four)
-        hipLaunchKernelGGL((append4_kernel<T>), grid, dim3(threads), 0, stream, p);
+        enqueue(p.inter ? append4_kernel<T, true> : append4_kernel<T, false>);
     else if (vw == 8)
-        hipLaunchKernelGGL((append_kernel<T, 8>), grid, dim3(threads), 0, stream, p);
+        enqueue(p.inter ? append_kernel<T, 8, true> : append_kernel<T, 8, false>);
     else
-        hipLaunchKernelGGL((append_kernel<T, 1>), grid, dim3(threads), 0, stream, p);
+        enqueue(p.inter ? append_kernel<T, 1, true> : append_kernel<T, 1, false>);
     return hipGetLastError();
 }
 
@@ -411,32 +572,58 @@ template <typename T, bool FOUR>
 __global__ __launch_bounds__(THREADS) void read_kernel(const ReadParams p) {
     const int unit = blockIdx.x / p.blocks;
     const int b = unit / p.c.hkv, h = unit - b * p.c.hkv;
-    const int i = (blockIdx.x - unit * p.blocks) * THREADS + threadIdx.x;
-    const int pos = fwd::fdiv(i, p.fd_chunks);
-    if (pos >= p.max_k) return;
-    int c = i - pos * (p.nk + p.nv);
-    const bool key = c < p.nk;
-    if (!key) c -= p.nk;
-    u32x4 out = u32x4{0u, 0u, 0u, 0u};
-    if (pos < min(max(uniform_i32(p.c.klen + b), 0), p.c.capacity)) {
-        int row = 0;
-        const int page = max(page_of(p.c, b, pos, row), 0);
-        const int64_t* st = key ? p.c.ks : p.c.vs;
-        const char* src = (key ? p.c.k : p.c.v) + page * st[0] + h * st[1] + row * st[2];
-        if constexpr (FOUR) {
-            const int64_t* sst = key ? p.c.kss : p.c.vss;
-            const uint8_t byte = (key ? p.c.ksc : p.c.vsc)[page * sst[0] + h * sst[1] + row * sst[2] + (c >> 2)];
-            const uint32_t codes = *reinterpret_cast<const uint32_t*>(src + 4 * c);
-            const float s = scale_of(byte);
+    const int first = (blockIdx.x - unit * p.blocks) * (THREADS * ITEMS) + threadIdx.x;
+    const int lk = min(max(uniform_i32(p.c.klen + b), 0), p.c.capacity);
+    u32x4 x[ITEMS];
+    uint32_t byte[ITEMS];
+    int pos[ITEMS], c[ITEMS], entry[ITEMS], row[ITEMS];
+    bool key[ITEMS];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) out[j] = fp4_pair<T>(codes, s, j);
-        } else {
-            out = *reinterpret_cast<const u32x4*>(src + 16 * c);
+    for (int j = 0; j < ITEMS; ++j) {
+        pos[j] = fwd::fdiv(first + j * THREADS, p.fd_chunks);
+        c[j] = first + j * THREADS - pos[j] * (p.nk + p.nv);
+        key[j] = c[j] < p.nk;
+        if (!key[j]) c[j] -= p.nk;
+        x[j] = u32x4{0u, 0u, 0u, 0u};
+        byte[j] = 0;
+    }
+    if (lk > 0) {
+        // Every table entry, then every row (keys past the last repeat its, unused), so that a
+        // thread's items wait for memory together.
+#pragma unroll
+        for (int j = 0; j < ITEMS; ++j) {
+            const int at = min(pos[j], lk - 1), n = fwd::fdiv(at, p.c.fd_page);
+            row[j] = at - n * p.c.page;
+            entry[j] = p.c.table[b * p.c.table_stride + n];
+        }
+#pragma unroll
+        for (int j = 0; j < ITEMS; ++j) {
+            const int page = clamp_page(entry[j], p.c.pages);
+            const char* src = key[j] ? p.c.k + page * p.c.ks[0] + h * p.c.ks[1] + row[j] * p.c.ks[2]
+                                     : p.c.v + page * p.c.vs[0] + h * p.c.vs[1] + row[j] * p.c.vs[2];
+            if constexpr (FOUR) {
+                const uint8_t* sc = key[j] ? p.c.ksc + page * p.c.kss[0] + h * p.c.kss[1] + row[j] * p.c.kss[2]
+                                           : p.c.vsc + page * p.c.vss[0] + h * p.c.vss[1] + row[j] * p.c.vss[2];
+                byte[j] = sc[c[j] >> 2];
+                x[j][0] = *reinterpret_cast<const uint32_t*>(src + 4 * c[j]);
+            } else {
+                x[j] = *reinterpret_cast<const u32x4*>(src + 16 * c[j]);
+            }
         }
     }
-    char* dst = static_cast<char*>(key ? p.k : p.v);
-    const int n = key ? p.nk : p.nv;
-    *reinterpret_cast<u32x4*>(dst + ((static_cast<int64_t>(unit) * p.max_k + pos) * n + c) * 16) = out;
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) {
+        if (pos[j] >= p.max_k) continue;
+        if constexpr (FOUR) {
+            const uint32_t codes = x[j][0];
+            const float s = scale_of(byte[j]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[j][e] = fp4_pair<T>(codes, s, e);
+        }
+        if (pos[j] >= lk) x[j] = u32x4{0u, 0u, 0u, 0u};
+        char* dst = static_cast<char*>(key[j] ? p.k : p.v);
+        *reinterpret_cast<u32x4*>(dst + ((static_cast<int64_t>(unit) * p.max_k + pos[j]) * (key[j] ? p.nk : p.nv) + c[j]) * 16) = x[j];
+    }
 }
 
 }  // namespace
@@ -450,7 +637,7 @@ hipError_t launch_read(const kmi_paged_cache& cache, void* k, void* v, int64_t m
     p.nk = p.c.d / 8;
     p.nv = p.c.dv / 8;
     p.fd_chunks = fwd::fast_div(static_cast<uint32_t>(p.nk + p.nv));
-    p.blocks = static_cast<int>(ceil_div(max_k * (p.nk + p.nv), THREADS));
+    p.blocks = static_cast<int>(ceil_div(max_k * (p.nk + p.nv), THREADS * ITEMS));
     const dim3 grid(static_cast<unsigned>(p.blocks * cache.batch * cache.heads_kv));
     const bool bf = cache.dtype == KMI_BF16;
     if (cache.bits == 4) {
@@ -470,9 +657,9 @@ hipError_t launch_read(const kmi_paged_cache& cache, void* k, void* v, int64_t m
 // (HIP's limit of 2^32 threads) and a unit's chunks below 2^31.
 bool read_fits(const kmi_paged_cache& c, int64_t max_k) {
     const int64_t per = c.head_dim / 8 + c.head_dim_v / 8;
-    if (max_k > ((int64_t{1} << 31) - THREADS) / per) return false;
+    if (max_k > ((int64_t{1} << 31) - THREADS * ITEMS) / per) return false;
     const int64_t units = c.batch * c.heads_kv;
-    return units == 0 || ceil_div(max_k * per, THREADS) < (int64_t{1} << 24) / units;
+    return units == 0 || ceil_div(max_k * per, THREADS * ITEMS) < (int64_t{1} << 24) / units;
 }
 
 }  // namespace paged

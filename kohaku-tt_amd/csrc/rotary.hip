@@ -1,12 +1,14 @@
 // Rotary positions (kmi_rotary): pairs of a head's dims turned by the angle position *
 // inv_freq, forward and (by the opposite angle) backward.
 //
-// Bound by memory: every value is read and written once, for three operations.  A thread
-// owns V pairs (one 16-byte vector of each half; two adjacent vectors when interleaved) of one
-// token, forms their sines and cosines once (about 45 instructions a pair, the angles in 64
-// bits) and walks its share of the token's heads with them, four heads' loads in flight.
-// Few tokens spread their heads over more threads instead, since nothing is gained by sharing
-// angles when most of the chip idles.
+// Bound by memory: every value is read and written once, for three operations.  A workgroup owns
+// a few tokens.  Its threads first request their vectors (a pair of 16-byte vectors of one head
+// each: one of each half, or two adjacent ones when interleaved), then form the tokens' sines and
+// cosines into LDS, one pair a thread (about 45 instructions, the angles in 64 bits, behind the
+// loads' latency), and then turn and store.  Angles are so formed once per token and not per
+// head, and no thread walks the heads one after the other.
+#include <algorithm>
+
 #include "paged.hpp"
 
 namespace kmi {
@@ -26,11 +28,10 @@ struct Params {
     const float* freq;
     float scale;
     int inverse;
-    int hg;       // threads that share a token's chunk, each with every hg-th head
     int chunks;   // of a head: rotated pairs of vectors, then copied vectors
-    int tpt;      // threads of a token: hg * chunks
+    int per;      // items (pairs of vectors, copied vectors) of a token: heads * chunks
     int tpb;      // tokens of a workgroup
-    fwd::FastDiv fd_tpt, fd_chunks;
+    fwd::FastDiv fd_seq, fd_half, fd_chunks, fd_per;
 };
 
 template <typename T, int V>
@@ -56,89 +57,92 @@ __device__ __forceinline__ void store(T* p, const Vec<T, V>& v) {
 }
 
 constexpr int THREADS = 256;
-constexpr int BATCH = 4;  // heads in flight
+constexpr int ITEMS = 4;       // of a thread, in flight together
+constexpr int PAIRS = 2048;    // angles of a workgroup
 
 template <typename T, int V, bool INTER>
 __global__ __launch_bounds__(THREADS) void rotary_kernel(const Params p) {
-    const int tl = fwd::fdiv(threadIdx.x, p.fd_tpt);
-    if (tl >= p.tpb) return;
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * p.tpb + tl;
-    if (t >= p.tokens) return;
-    const int rem = threadIdx.x - tl * p.tpt;
-    const int hg = fwd::fdiv(rem, p.fd_chunks), c = rem - hg * p.chunks;
-    const int64_t b = t / p.seq, s = t - b * p.seq;
-    const int nrot = p.rd / (2 * V);
-    const bool rot = c < nrot;
-    // First and second vector of the chunk (a copied chunk has one).
-    const int lo = rot ? (INTER ? 2 * V * c : V * c) : p.rd + V * (c - nrot);
-    const int hi = rot ? (INTER ? lo + V : lo + p.rd / 2) : lo;
-    const int heads = p.heads[0] + p.heads[1];
-    auto src = [&](int h) {
-        const int w = h >= p.heads[0];
-        return static_cast<const T*>(p.x[w]) + b * p.xs[w][0] + (h - (w ? p.heads[0] : 0)) * p.xs[w][1] + s * p.xs[w][2];
-    };
-    auto dst = [&](int h) {
-        const int w = h >= p.heads[0];
-        return static_cast<T*>(p.y[w]) + b * p.ys[w][0] + (h - (w ? p.heads[0] : 0)) * p.ys[w][1] + s * p.ys[w][2];
-    };
-    Vec<T, V> a[BATCH], z[BATCH];
-    auto fetch = [&](int h0) {
+    __shared__ __align__(16) float cosine[PAIRS], sine[PAIRS];
+    const int t0 = blockIdx.x * p.tpb;
+    const int nt = min(p.tpb, static_cast<int>(p.tokens) - t0);
+    const int half = p.rd / 2, nrot = half / V;
+    const int items = nt * p.per;
+    // An item's vectors and its first angle (negative: copied).
+    Vec<T, V> a[ITEMS], z[ITEMS];
+    T* dst[ITEMS];
+    int lo[ITEMS], hi[ITEMS], at[ITEMS];
+    auto fetch = [&](int base) {
 #pragma unroll
-        for (int j = 0; j < BATCH; ++j) {
-            const int h = h0 + j * p.hg;
-            if (h < heads) {
-                const T* x = src(h);
-                a[j] = load<T, V>(x + lo);
-                if (rot) z[j] = load<T, V>(x + hi);
-            }
+        for (int j = 0; j < ITEMS; ++j) {
+            const int i = base + j * THREADS + threadIdx.x;
+            if (i >= items) continue;
+            const int tl = fwd::fdiv(i, p.fd_per), r = i - tl * p.per;
+            int h = fwd::fdiv(r, p.fd_chunks);
+            const int c = r - h * p.chunks;
+            const int w = h >= p.heads[0];
+            h -= w ? p.heads[0] : 0;
+            const int b = fwd::fdiv(t0 + tl, p.fd_seq), s = t0 + tl - b * p.seq;
+            const T* x = static_cast<const T*>(p.x[w]) + b * p.xs[w][0] + h * p.xs[w][1] + s * p.xs[w][2];
+            dst[j] = static_cast<T*>(p.y[w]) + b * p.ys[w][0] + h * p.ys[w][1] + s * p.ys[w][2];
+            const bool rot = c < nrot;
+            lo[j] = rot ? (INTER ? 2 * V * c : V * c) : p.rd + V * (c - nrot);
+            hi[j] = INTER ? lo[j] + V : lo[j] + half;
+            at[j] = rot ? tl * half + V * c : -1;
+            a[j] = load<T, V>(x + lo[j]);
+            if (rot) z[j] = load<T, V>(x + hi[j]);
         }
     };
-    fetch(hg);  // (before the angles, whose latency it hides)
-    float cs[V], sn[V];
-    if (rot) {
-        const int64_t at = b * p.ps[0] + s * p.ps[1];
-        const double pos = p.wide ? static_cast<double>(static_cast<const int64_t*>(p.positions)[at])
-                                  : static_cast<double>(static_cast<const int32_t*>(p.positions)[at]);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            paged::turn(pos, p.freq[V * c + i], cs[i], sn[i]);
-            cs[i] *= p.scale;
-            sn[i] *= p.inverse ? -p.scale : p.scale;
-        }
+    fetch(0);
+    for (int i = threadIdx.x; i < nt * half; i += THREADS) {
+        const int tl = fwd::fdiv(i, p.fd_half), k = i - tl * half;
+        const int b = fwd::fdiv(t0 + tl, p.fd_seq), s = t0 + tl - b * p.seq;
+        const int64_t n = b * p.ps[0] + s * p.ps[1];
+        const double pos = p.wide ? static_cast<double>(static_cast<const int64_t*>(p.positions)[n])
+                                  : static_cast<double>(static_cast<const int32_t*>(p.positions)[n]);
+        float c, sn;
+        paged::turn(pos, p.freq[k], c, sn);
+        cosine[i] = c * p.scale;
+        sine[i] = sn * (p.inverse ? -p.scale : p.scale);
     }
-    for (int h0 = hg; h0 < heads; h0 += BATCH * p.hg) {
+    __syncthreads();
+    for (int base = 0;;) {
 #pragma unroll
-        for (int j = 0; j < BATCH; ++j) {
-            const int h = h0 + j * p.hg;
-            if (h >= heads) break;
-            T* y = dst(h);
-            if (!rot) {
-                store<T, V>(y + lo, a[j]);
+        for (int j = 0; j < ITEMS; ++j) {
+            if (base + j * THREADS + static_cast<int>(threadIdx.x) >= items) break;
+            if (at[j] < 0) {
+                store<T, V>(dst[j] + lo[j], a[j]);
                 continue;
             }
+            float cs[V], sn[V];
+            __builtin_memcpy(cs, __builtin_assume_aligned(cosine + at[j], V * 4), V * 4);
+            __builtin_memcpy(sn, __builtin_assume_aligned(sine + at[j], V * 4), V * 4);
             Vec<T, V> u, w;
             if constexpr (INTER && V > 1) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    Vec<T, V>& in = i < V / 2 ? a[j] : z[j];
+                    const Vec<T, V>& in = i < V / 2 ? a[j] : z[j];
                     Vec<T, V>& out = i < V / 2 ? u : w;
                     const int k = 2 * (i % (V / 2));
-                    const float x1 = to_f32(in.e[k]), x2 = to_f32(in.e[k + 1]);
-                    out.e[k] = from_f32<T>(x1 * cs[i] - x2 * sn[i]);
-                    out.e[k + 1] = from_f32<T>(x2 * cs[i] + x1 * sn[i]);
+                    float y1, y2;
+                    paged::turned(to_f32(in.e[k]), to_f32(in.e[k + 1]), cs[i], sn[i], y1, y2);
+                    out.e[k] = from_f32<T>(y1);
+                    out.e[k + 1] = from_f32<T>(y2);
                 }
             } else {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float x1 = to_f32(a[j].e[i]), x2 = to_f32(z[j].e[i]);
-                    u.e[i] = from_f32<T>(x1 * cs[i] - x2 * sn[i]);
-                    w.e[i] = from_f32<T>(x2 * cs[i] + x1 * sn[i]);
+                    float y1, y2;
+                    paged::turned(to_f32(a[j].e[i]), to_f32(z[j].e[i]), cs[i], sn[i], y1, y2);
+                    u.e[i] = from_f32<T>(y1);
+                    w.e[i] = from_f32<T>(y2);
                 }
             }
-            store<T, V>(y + lo, u);
-            store<T, V>(y + hi, w);
+            store<T, V>(dst[j] + lo[j], u);
+            store<T, V>(dst[j] + hi[j], w);
         }
-        if (h0 + BATCH * p.hg < heads) fetch(h0 + BATCH * p.hg);
+        base += ITEMS * THREADS;
+        if (base >= items) break;
+        fetch(base);
     }
 }
 
@@ -188,15 +192,14 @@ hipError_t launch(const kmi_rotary_args* a, hipStream_t stream) {
     p.inverse = a->inverse ? 1 : 0;
     const int v = vec ? W : 1;
     p.chunks = p.rd / (2 * v) + (p.d - p.rd) / v;
-    // Threads per token: enough for two wavefronts per SIMD over the chip when there are few
-    // tokens, else one thread for all heads of a chunk.
-    const int heads = p.heads[0] + p.heads[1];
-    p.hg = 1;
-    while (2 * p.hg * p.chunks <= THREADS && p.hg < heads && p.tokens * p.chunks * p.hg < (1 << 17)) p.hg *= 2;
-    p.tpt = p.hg * p.chunks;
-    p.tpb = THREADS / p.tpt;
-    p.fd_tpt = fwd::fast_div(static_cast<uint32_t>(p.tpt));
+    p.per = (p.heads[0] + p.heads[1]) * p.chunks;
+    // Tokens of a workgroup: a batch of items a thread, unless few tokens leave CUs idle.
+    const int64_t fill = std::min<int64_t>(ITEMS * THREADS / p.per, PAIRS / (p.rd / 2));
+    p.tpb = static_cast<int>(std::max<int64_t>(1, std::min(fill, p.tokens / 1024)));
+    p.fd_seq = fwd::fast_div(static_cast<uint32_t>(p.seq));
+    p.fd_half = fwd::fast_div(static_cast<uint32_t>(p.rd / 2));
     p.fd_chunks = fwd::fast_div(static_cast<uint32_t>(p.chunks));
+    p.fd_per = fwd::fast_div(static_cast<uint32_t>(p.per));
     const dim3 grid(static_cast<unsigned>(ceil_div(p.tokens, p.tpb)));
     if (vec) {
         if (a->interleaved)
