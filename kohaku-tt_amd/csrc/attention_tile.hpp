@@ -98,8 +98,7 @@ __device__ __forceinline__ void attn_tile(const P& p, unsigned char* smem, const
         lq = min(span.lq, p.seq_q);
         lall = span.lk;
         const int per = p.split_keys(lall, KT);
-        s0 = split * per;
-        if (split > 0 && s0 >= lall) return;  // (split 0 writes the rows of a sequence without keys)
+        s0 = min(split * per, lall);
         lk = min(lall - s0, per);
     } else if (p.cu_q) {
         q0 = min(max(p.cu_q[seq], 0), p.total_q);
@@ -537,7 +536,7 @@ __device__ __forceinline__ void attn_tile(const P& p, unsigned char* smem, const
     if (row >= vrows) return;
     const float inv = l > 0.f ? 1.f / l : 0.f;
     if constexpr (PAGED) {
-        if (p.split_keys(lall, KT) < lall) {
+        if (p.splits > 1) {
             // One of several splits: normalised rows and base-2 log-sum-exps, merged by a launch
             // of their own.
             const int64_t at = (static_cast<int64_t>(split) * p.rows_total + q0 + pos) * p.hq + head;

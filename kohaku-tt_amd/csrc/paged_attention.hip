@@ -71,8 +71,13 @@ Plan make_plan(const kmi_paged_attn_args* a) {
         pl.decode = true;
         pl.rows = vrows <= 16 ? 16 : 32;
         pl.nx = 1;
-        pl.min_split = 4 * kDecodeTile;
-        splits = ceil_div(1024, std::max<int64_t>(1, units));
+        // Two workgroups of four wavefronts per CU, a tile for each of a split's wavefronts and
+        // two where there are many splits (us at 4, 7 / 20, 40 splits: 14/2 heads x 777 keys x 64
+        // 8.1, 6.6; 4 bits, 3 x 4 tokens over 5001 keys 11.7, 12.3; 64 sequences x 2 heads x 8192
+        // keys x 128, at 2, 4, 6, 8 splits 100, 101, 103, 103, in 4 bits 52.5, 39.1, 38.9, 44.4).
+        pl.min_split = kDecodeTile;
+        splits = std::min(ceil_div(512, std::max<int64_t>(1, units)),
+                          std::max(std::min<int64_t>(ceil_div(keys, 4 * kDecodeTile), 8), keys / (8 * kDecodeTile)));
     } else {
         const int64_t w4 = ceil_div(vrows, 128) * units;
         pl.row_groups = pl.dp <= 128 && w4 >= 448 ? 4 : 2;
@@ -92,39 +97,48 @@ Plan make_plan(const kmi_paged_attn_args* a) {
     return pl;
 }
 
-// One wavefront per (query token, query head) of a split sequence: the splits' normalised rows
-// weighted by their sums.
+// One wavefront per (query token, query head): the splits' normalised rows weighted by their sums.
+// Nothing is looked up (every split of every row wrote its log-sum-exp), so the first rows are
+// requested beside the sums: one memory round trip.  Rows of empty splits are read and dropped.
+constexpr int MERGE_ROWS = 4;   // of a workgroup
+constexpr int MERGE_BATCH = 8;  // splits in flight
 template <typename T, int DP>
-__global__ __launch_bounds__(kWave) void merge_kernel(const AttnParams p, const int unit_keys, const int row_blocks) {
+__global__ __launch_bounds__(MERGE_ROWS * kWave) void merge_kernel(const AttnParams p) {
     constexpr int E = DP <= 64 ? 1 : (DP <= 128 ? 2 : 4);  // dims of a lane (value head dims are multiples of 8)
-    const int bh = blockIdx.x / row_blocks, r = blockIdx.x - bh * row_blocks;
-    const int seq = fwd::fdiv(bh, p.fd_hkv), kvh = bh - seq * p.hkv;
-    const Span sp = p.span(seq);
-    if (r >= min(sp.lq, p.seq_q) * p.group) return;
-    const int per = p.split_keys(sp.lk, unit_keys);
-    if (per >= sp.lk) return;  // one split: its workgroup wrote the output
-    const int n = (sp.lk + per - 1) / per;
-    const int pos = fwd::fdiv(r, p.fd_group), head = kvh * p.group + (r - pos * p.group);
-    const int64_t tok = sp.q0 + pos, row = tok * p.hq + head, step = p.rows_total * p.hq;
-    const int lane = threadIdx.x, d0 = lane * E;
-    const float lse = lane < n ? p.part_lse[lane * step + row] : -INFINITY;
+    const int64_t step = p.rows_total * p.hq;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * MERGE_ROWS + (threadIdx.x >> 6);
+    if (row >= step) return;
+    const int lane = threadIdx.x & 63, d0 = lane * E, dc = min(d0, p.dv - E);
+    struct Vec {
+        float e[E];
+    };
+    const float* src = p.part_o + row * DP + dc;
+    Vec x[MERGE_BATCH];
+    auto fetch = [&](int s0) {
+#pragma unroll
+        for (int s = 0; s < MERGE_BATCH; ++s)
+            __builtin_memcpy(&x[s], __builtin_assume_aligned(src + min(s0 + s, p.splits - 1) * step * DP, E * 4), E * 4);
+    };
+    fetch(0);
+    const float lse = lane < p.splits ? p.part_lse[lane * step + row] : -INFINITY;
     const float top = wave_max(lse);
     const float w = lse == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(lse - top);
     const float total = wave_sum(w);
-    const float inv = total > 0.f ? 1.f / total : 0.f;
     float acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    if (d0 < p.dv) {
-        const float* src = p.part_o + row * DP + d0;
-#pragma unroll 8
-        for (int s = 0; s < n; ++s) {
-            const float ws = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), s));
-            float x[E];
-            __builtin_memcpy(x, __builtin_assume_aligned(src + s * step * DP, E * 4), E * 4);
+    for (int s0 = 0; s0 < p.splits; s0 += MERGE_BATCH) {
+        if (s0 > 0) fetch(s0);
 #pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] += ws * x[e];
+        for (int s = 0; s < MERGE_BATCH; ++s) {
+            const float ws = s0 + s < p.splits ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), s0 + s)) : 0.f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] += ws > 0.f ? ws * x[s].e[e] : 0.f;  // (never written where 0)
         }
+    }
+    const int tok = static_cast<int>(row / p.hq), head = static_cast<int>(row - static_cast<int64_t>(tok) * p.hq);
+    if (d0 < p.dv) {
+        const float inv = total > 0.f ? 1.f / total : 0.f;
         T y[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) y[e] = from_f32<T>(acc[e] * inv);
@@ -140,11 +154,9 @@ hipError_t run(const AttnParams& p, const Plan& pl, bool four, hipStream_t strea
     const hipError_t err = pl.decode ? launch_decode<T, DP>(p, pl.rows, four, stream)
                                      : launch_tile<T, DP>(p, pl.row_groups, stream);
     if (err != hipSuccess || pl.splits == 1) return err;
-    // (The tile kernel's key tiles: 128 for two row groups up to head dim 64, else 64.)
-    const int unit = pl.decode ? kDecodeTile : (DP <= 64 && pl.row_groups == 2 ? 128 : 64);
-    const int rows = p.seq_q * p.group;
-    hipLaunchKernelGGL((merge_kernel<T, DP>), dim3(static_cast<unsigned>(p.batch * p.hkv * rows)), dim3(kWave), 0, stream, p,
-                       unit, rows);
+    const int64_t rows = p.rows_total * p.hq;
+    hipLaunchKernelGGL((merge_kernel<T, DP>), dim3(static_cast<unsigned>(ceil_div(rows, MERGE_ROWS))),
+                       dim3(MERGE_ROWS * kWave), 0, stream, p);
     return hipGetLastError();
 }
 
@@ -164,8 +176,8 @@ hipError_t run_dim(const AttnParams& p, const Plan& pl, bool four, hipStream_t s
 bool grid_fits(const kmi_paged_attn_args* a, const Plan& pl) {
     const double units = static_cast<double>(a->cache.batch) * a->cache.heads_kv;
     const double blocks = units * pl.nx * pl.splits;
-    const double rows = pl.splits > 1 ? units * a->max_q * (a->heads_q / a->cache.heads_kv) : 0.0;
-    return blocks < (1 << 24) - 1 && rows < (1 << 26);
+    const double rows = static_cast<double>(a->cache.tokens) * a->heads_q;
+    return blocks < (1 << 23) - 1 && (pl.splits == 1 || rows < (1 << 26));
 }
 
 }  // namespace
@@ -207,6 +219,11 @@ extern "C" int kmi_paged_attn(const kmi_paged_attn_args* a, void* workspace, siz
     AttnParams p{};
     p.c = device_cache(a->cache);
     p.c.capacity = static_cast<int>(keys);
+    if (keys == 0) {
+        // No table entry can be read: any int32 stands for the first one, and no key is.
+        p.c.table = a->cache.key_lengths;
+        p.c.table_stride = 0;
+    }
     const bool copy = pl.copy_bytes > 0;
     if (copy) {
         if (!read_fits(a->cache, keys)) return fail(KMI_EINVAL, "kmi_paged_attn: max_k out of range");

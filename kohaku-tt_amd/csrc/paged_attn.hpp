@@ -15,8 +15,7 @@ struct AttnParams : fwd::AttnParams {
     int head_pages;    // 1: c.k / c.v are dense copies [batch, heads_kv, capacity, dim] (no table)
     __device__ __forceinline__ Span span(int seq) const { return span_of(c, seq); }
     // Keys of a split of a sequence with `lk` keys, a multiple of `unit`: the sequence in at most
-    // `splits` parts of at least min_split.  Every kernel and the merge derive it alike, so
-    // nothing but the partials passes between them.
+    // `splits` parts of at least min_split; splits past the last key write empty partials.
     __device__ __forceinline__ int split_keys(int lk, int unit) const {
         const int per = fwd::fdiv(lk + splits - 1, fd_splits);
         return max((max(per, min_split) + unit - 1) / unit * unit, unit);
@@ -43,14 +42,21 @@ struct AttnParams : fwd::AttnParams {
     }
 };
 
-// Zeros (and log-sum-exps of minus infinity) for the rows behind the last sequence: one
-// workgroup of a call does it.
+// Zeros (and log-sum-exps of minus infinity) for the rows behind the last sequence, in a split
+// call through the merge: one workgroup of a call does it.
 template <typename T>
 __device__ __forceinline__ void zero_tail(const AttnParams& p) {
     if (!p.c.cu) return;
     const int t0 = min(max(uniform_i32(p.c.cu + p.c.batch), 0), p.c.tokens);
     const int vec = p.dv / 4;
     const int64_t n = static_cast<int64_t>(p.c.tokens - t0) * p.hq;
+    if (p.splits > 1) {
+        for (int64_t i = threadIdx.x; i < n * p.splits; i += blockDim.x) {
+            const int64_t s = i / n;
+            p.part_lse[(s * p.rows_total + t0) * p.hq + (i - s * n)] = -INFINITY;
+        }
+        return;
+    }
     typedef T t4 __attribute__((ext_vector_type(4)));
     for (int64_t i = threadIdx.x; i < n * vec; i += blockDim.x) {
         const int64_t r = i / vec, t = t0 + r / p.hq, h = r % p.hq;

@@ -45,6 +45,10 @@ const char* check_cache(const kmi_paged_cache& c, bool uses_tokens) {
     if (c.k_stride[2] > (1 << 24) || c.v_stride[2] > (1 << 24) ||
         (c.bits == 4 && (c.k_scale_stride[2] > (1 << 24) || c.v_scale_stride[2] > (1 << 24))))
         return "cache row strides must be at most 2^24";
+    // (A page's offset is the product of two 32-bit numbers.)
+    for (const int64_t* st : {c.k_stride, c.v_stride, c.k_scale_stride, c.v_scale_stride})
+        if ((c.bits == 4 || (st != c.k_scale_stride && st != c.v_scale_stride)) && st[0] > INT32_MAX / 2)
+            return "cache page strides must be below 2^30";
     if (c.batch < 0 || c.batch > (1 << 24)) return "batch out of range";
     if (c.table_width < 0 || (c.table_width > 1 && c.table_stride < 0)) return "bad block_table strides";
     if (c.table_width > (int64_t{1} << 30) / c.page_size) return "block_table holds more than 2^30 keys a sequence";

@@ -88,7 +88,7 @@ constexpr int v_pitch(int dp) { return dp + 16; }
 template <typename T, int DP, int NQ>
 constexpr size_t decode_lds() {
     const size_t v = static_cast<size_t>(WAVES) * TK * v_pitch(DP) * sizeof(T);
-    const size_t merge = static_cast<size_t>(2) * NQ * 16 * (DP + 4) * sizeof(float) + 2 * NQ * 16 * 2 * sizeof(float);
+    const size_t merge = static_cast<size_t>(WAVES) * 16 * (DP + 4 + 2) * sizeof(float);
     return v > merge ? v : merge;
 }
 
@@ -100,6 +100,7 @@ __global__ __launch_bounds__(THREADS) void paged_decode_kernel(const AttnParams 
     constexpr int DB = DP / 16;                // output blocks
     constexpr int VP = v_pitch(DP);
     constexpr int CP = DP + 4;
+    constexpr int DEPTH = FOUR ? 2 : 1;  // tiles of a wavefront in flight
     // V staging, 16 bits: VPS lanes a row (a power of two; those past the padded row idle).
     constexpr int NCH = DP / 8;
     constexpr int VPS = NCH <= 4 ? 4 : NCH <= 8 ? 8 : NCH <= 16 ? 16 : 32;
@@ -120,14 +121,122 @@ __global__ __launch_bounds__(THREADS) void paged_decode_kernel(const AttnParams 
     const int split = blockIdx.x - bh * p.splits;
     const int seq = fwd::fdiv(bh, p.fd_hkv), kvh = bh - seq * p.hkv;
     const int G = p.group;
+    // Tiles are dealt to a unit's wavefronts in turn: tile slot, slot + nslots, ...  A wavefront's
+    // first table entries are so known before the sequence's length, and read beside it.
+    const int slot = split * WAVES + wave, nslots = p.splits * WAVES;
+
+    // Tiles in registers.
+    struct TileRegs {
+        v8 k[FOUR ? 1 : 2][FOUR ? 1 : DC];
+        u32x4 v[FOUR ? 1 : 2][FOUR ? 1 : KIT];
+        u32x4 k4[FOUR ? 2 : 1][FOUR ? KC : 1], v4[FOUR ? 2 : 1][FOUR ? R4 : 1];
+        uint32_t k4s[FOUR ? 2 : 1][FOUR ? KC : 1], v4s[FOUR ? 2 : 1][FOUR ? R4 : 1];
+    };
+    TileRegs reg[DEPTH];
+    T* const vl = reinterpret_cast<T*>(smem) + wave * TK * VP;
+    const int krow = lane / VPS, dg = lane % VPS;
+    const uint32_t kst = static_cast<uint32_t>(p.c.ks[2]), vst = static_cast<uint32_t>(p.c.vs[2]);
+    const uint32_t kss = FOUR ? static_cast<uint32_t>(p.c.kss[2]) : 0, vss = FOUR ? static_cast<uint32_t>(p.c.vss[2]) : 0;
+    // The unit's head within a page.
+    const char* const kh = p.c.k + kvh * p.c.ks[1];
+    const char* const vh = p.c.v + kvh * p.c.vs[1];
+    const uint8_t* const ksh = FOUR ? p.c.ksc + kvh * p.c.kss[1] : nullptr;
+    const uint8_t* const vsh = FOUR ? p.c.vsc + kvh * p.c.vss[1] : nullptr;
+
+    // The page and row of a half tile (keys past what the table holds repeat its last).
+    struct Entry {
+        int page, row;
+    };
+    auto entry = [&](int key) {
+        Entry e;
+        e.page = p.page_at(seq, max(min(key, p.c.capacity - 1), 0), e.row);
+        return e;
+    };
+    // (Page strides are below 2^32 bytes.)
+    auto at = [](const auto* base, const Entry& e, int64_t page_stride, uint32_t row_stride) {
+        return base + static_cast<uint64_t>(static_cast<uint32_t>(e.page)) * static_cast<uint32_t>(page_stride) +
+               static_cast<uint32_t>(e.row) * static_cast<uint64_t>(row_stride);
+    };
+    // The lane's byte offsets within a half (past every range for dims that are none).
+    uint32_t koff[FOUR ? KC : DC], voff[FOUR ? R4 : 1], ksoff[FOUR ? KC : 1], vsoff[FOUR ? R4 : 1];
+    if constexpr (!FOUR) {
+#pragma unroll
+        for (int c = 0; c < DC; ++c) koff[c] = 32 * c + 8 * g4 < p.d ? l16 * kst + 16 * g4 + 64 * c : kNone;
+        voff[0] = 8 * dg < p.dv ? krow * vst + 16 * dg : kNone;
+    } else {
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+            const bool in = 128 * c + 32 * g4 < p.d;
+            koff[c] = in ? l16 * kst + 64 * c + 16 * g4 : kNone;
+            ksoff[c] = in ? l16 * kss + 4 * c + g4 : kNone;
+        }
+#pragma unroll
+        for (int i = 0; i < R4; ++i) {
+            const int ci = lane + kWave * i, r = ci / N4, ch = ci % N4;
+            const bool in = r < 16 && 32 * ch < p.dv;
+            voff[i] = in ? r * vst + 16 * ch : kNone;
+            vsoff[i] = in ? r * vss + ch : kNone;
+        }
+    }
+    // Requests `rows` rows (at most 16 n) from an entry on into halves h .. h + n - 1.
+    auto request = [&](TileRegs& x, const Entry& e, int rows, int h0, int n) __attribute__((always_inline)) {
+        const auto rk = buffer_rsrc(at(kh, e, p.c.ks[0], kst), rows_extent(rows, kst, FOUR ? p.d / 2 : 2 * p.d));
+        const auto rv = buffer_rsrc(at(vh, e, p.c.vs[0], vst), rows_extent(rows, vst, FOUR ? p.dv / 2 : 2 * p.dv));
+        if constexpr (!FOUR) {
+#pragma unroll
+            for (int h = 0; h < n; ++h) {
+#pragma unroll
+                for (int c = 0; c < DC; ++c)
+                    x.k[h0 + h][c] = __builtin_bit_cast(v8, buffer_load16(rk, koff[c] + 16 * h * kst));
+#pragma unroll
+                for (int i = 0; i < KIT; ++i) x.v[h0 + h][i] = buffer_load16(rv, voff[0] + (16 * h + i * RPP) * vst);
+            }
+        } else {
+            const auto rks = buffer_rsrc(at(ksh, e, p.c.kss[0], kss), rows_extent(rows, kss, p.d / 32));
+            const auto rvs = buffer_rsrc(at(vsh, e, p.c.vss[0], vss), rows_extent(rows, vss, p.dv / 32));
+#pragma unroll
+            for (int h = 0; h < n; ++h) {
+#pragma unroll
+                for (int c = 0; c < KC; ++c) {
+                    x.k4[h0 + h][c] = buffer_load16(rk, koff[c] + 16 * h * kst);
+                    x.k4s[h0 + h][c] = __builtin_amdgcn_raw_buffer_load_b8(rks, ksoff[c] + 16 * h * kss, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < R4; ++i) {
+                    x.v4[h0 + h][i] = buffer_load16(rv, voff[i] + 16 * h * vst);
+                    x.v4s[h0 + h][i] = __builtin_amdgcn_raw_buffer_load_b8(rvs, vsoff[i] + 16 * h * vss, 0, 0);
+                }
+            }
+        }
+    };
+    // A tile lies in one page where pages are whole tiles, else its halves each in one.
+    const bool whole = p.c.page % TK == 0;  // (uniform)
+    struct Entries {
+        Entry half[2];
+    };
+    auto look_up = [&](int t) __attribute__((always_inline)) {
+        Entries e;
+        e.half[0] = entry(TK * t);
+        e.half[1] = whole ? e.half[0] : entry(TK * t + 16);
+        return e;
+    };
+    Entries next[DEPTH];  // of the tiles to request next
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i) next[i] = look_up(slot + i * nslots);
     const Span sp = p.span(seq);
     const int vrows = min(min(sp.lq, p.seq_q) * G, 16 * NQ);
     const int lk = sp.lk;
-    const int per = p.split_keys(lk, TK);
-    // (Uniform.)  Split 0 writes the rows of a sequence without keys.
-    if (vrows <= 0 || (split > 0 && split * per >= lk)) return;
-    const bool alone = per >= lk;
-    const int t0 = split * (per / TK), t1 = min((lk + TK - 1) / TK, t0 + per / TK);
+    if (vrows <= 0) return;  // (uniform)
+    const int nt = (lk + TK - 1) / TK;
+    auto load_tile = [&](TileRegs& x, int t, const Entries& e) __attribute__((always_inline)) {
+        const int rows = lk - TK * t;
+        if (whole) {
+            request(x, e.half[0], min(rows, TK), 0, 2);
+        } else {
+            request(x, e.half[0], min(rows, 16), 0, 1);
+            request(x, e.half[1], min(rows - 16, 16), 1, 1);
+        }
+    };
 
     // This lane's rows: query position and head, and the keys they see.
     int pos[NQ], head[NQ], lim[NQ];
@@ -206,87 +315,37 @@ __global__ __launch_bounds__(THREADS) void paged_decode_kernel(const AttnParams 
         }
     }
 
-    // A tile in registers.
-    v8 kreg[FOUR ? 1 : 2][FOUR ? 1 : DC];
-    u32x4 vreg[FOUR ? 1 : 2][FOUR ? 1 : KIT];
-    u32x4 k4[FOUR ? 2 : 1][FOUR ? KC : 1], v4[FOUR ? 2 : 1][FOUR ? R4 : 1];
-    uint32_t k4s[FOUR ? 2 : 1][FOUR ? KC : 1], v4s[FOUR ? 2 : 1][FOUR ? R4 : 1];
-    T* const vl = reinterpret_cast<T*>(smem) + wave * TK * VP;
-    const int krow = lane / VPS, dg = lane % VPS;
-    const uint32_t kst = static_cast<uint32_t>(p.c.ks[2]), vst = static_cast<uint32_t>(p.c.vs[2]);
-
-    // Table entries of a tile's halves (keys past the last one repeat its page).
-    struct Entry {
-        int page[2], row[2];
-    };
-    auto entries = [&](int t) {
-        Entry e;
+    // The first tiles, and the entries of those behind them.
+    int t = slot;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) e.page[h] = p.page_at(seq, min(TK * t + 16 * h, lk - 1), e.row[h]);
-        return e;
-    };
-    auto load_tile = [&](int t, const Entry& e) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int rows = min(lk - TK * t - 16 * h, 16);
-            const char* kb = p.c.k + e.page[h] * p.c.ks[0] + kvh * p.c.ks[1] + e.row[h] * p.c.ks[2];
-            const char* vb = p.c.v + e.page[h] * p.c.vs[0] + kvh * p.c.vs[1] + e.row[h] * p.c.vs[2];
-            if constexpr (!FOUR) {
-                const auto rk = buffer_rsrc(kb, rows_extent(rows, kst, 2 * p.d));
-                const auto rv = buffer_rsrc(vb, rows_extent(rows, vst, 2 * p.dv));
-#pragma unroll
-                for (int c = 0; c < DC; ++c)
-                    kreg[h][c] = __builtin_bit_cast(
-                        v8, buffer_load16(rk, 32 * c + 8 * g4 < p.d ? l16 * kst + 16 * g4 + 64 * c : kNone));
-#pragma unroll
-                for (int i = 0; i < KIT; ++i)
-                    vreg[h][i] = buffer_load16(rv, 8 * dg < p.dv ? (krow + i * RPP) * vst + 16 * dg : kNone);
-            } else {
-                const uint8_t* ksb = p.c.ksc + e.page[h] * p.c.kss[0] + kvh * p.c.kss[1] + e.row[h] * p.c.kss[2];
-                const uint8_t* vsb = p.c.vsc + e.page[h] * p.c.vss[0] + kvh * p.c.vss[1] + e.row[h] * p.c.vss[2];
-                const uint32_t kss = static_cast<uint32_t>(p.c.kss[2]), vss = static_cast<uint32_t>(p.c.vss[2]);
-                const auto rk = buffer_rsrc(kb, rows_extent(rows, kst, p.d / 2));
-                const auto rv = buffer_rsrc(vb, rows_extent(rows, vst, p.dv / 2));
-                const auto rks = buffer_rsrc(ksb, rows_extent(rows, kss, p.d / 32));
-                const auto rvs = buffer_rsrc(vsb, rows_extent(rows, vss, p.dv / 32));
-#pragma unroll
-                for (int c = 0; c < KC; ++c) {
-                    const bool in = 128 * c + 32 * g4 < p.d;
-                    k4[h][c] = buffer_load16(rk, in ? l16 * kst + 64 * c + 16 * g4 : kNone);
-                    k4s[h][c] = __builtin_amdgcn_raw_buffer_load_b8(rks, in ? l16 * kss + 4 * c + g4 : kNone, 0, 0);
-                }
-#pragma unroll
-                for (int i = 0; i < R4; ++i) {
-                    const int ci = lane + kWave * i, r = ci / N4, ch = ci % N4;
-                    const bool in = r < 16 && 32 * ch < p.dv;
-                    v4[h][i] = buffer_load16(rv, in ? r * vst + 16 * ch : kNone);
-                    v4s[h][i] = __builtin_amdgcn_raw_buffer_load_b8(rvs, in ? r * vss + ch : kNone, 0, 0);
-                }
-            }
+    for (int i = 0; i < DEPTH; ++i)
+        if (t + i * nslots < nt) {
+            load_tile(reg[i], t + i * nslots, next[i]);
+            next[i] = look_up(t + (i + DEPTH) * nslots);
         }
-    };
+
     // The tile's V rows into the wavefront's LDS.
-    auto stage = [&] {
+    auto stage = [&](const TileRegs& x) __attribute__((always_inline)) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             if constexpr (!FOUR) {
                 if (dg < NCH) {
 #pragma unroll
                     for (int i = 0; i < KIT; ++i)
-                        *reinterpret_cast<u32x4*>(vl + (16 * h + krow + i * RPP) * VP + 8 * dg) = vreg[h][i];
+                        *reinterpret_cast<u32x4*>(vl + (16 * h + krow + i * RPP) * VP + 8 * dg) = x.v[h][i];
                 }
             } else {
 #pragma unroll
                 for (int i = 0; i < R4; ++i) {
                     const int ci = lane + kWave * i, r = ci / N4, ch = ci % N4;
                     if (16 * N4 % kWave != 0 && r >= 16) continue;
-                    const float s = scale_of(v4s[h][i]);
+                    const float s = scale_of(x.v4s[h][i]);
                     T* dst = vl + (16 * h + r) * VP + 32 * ch;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         u32x4 w;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) w[e] = fp4_pair<T>(v4[h][i][j], s, e);
+                        for (int e = 0; e < 4; ++e) w[e] = fp4_pair<T>(x.v4[h][i][j], s, e);
                         *reinterpret_cast<u32x4*>(dst + 8 * j) = w;
                     }
                 }
@@ -304,18 +363,13 @@ __global__ __launch_bounds__(THREADS) void paged_decode_kernel(const AttnParams 
         neg_m[n] = lsum[n] = 0.f;
     }
 
-    int t = t0 + wave;
-    Entry next{};
-    if (t < t1) {
-        const Entry first = entries(t);
-        if (t + WAVES < t1) next = entries(t + WAVES);
-        load_tile(t, first);
-    }
-    for (; t < t1; t += WAVES) {
+    // A tile's products, softmax and PV; once its K operands are consumed, the tile DEPTH steps on
+    // is requested into its registers.
+    auto work = [&](TileRegs& x, Entries& e, int t) __attribute__((always_inline)) {
         // LDS keeps one wavefront's accesses in order (the previous tile's reads, these writes,
         // this tile's reads): only the compiler must keep it.
         __asm__ volatile("" ::: "memory");
-        stage();
+        stage(x);
         f32x4 s[NQ][2];
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
@@ -324,24 +378,24 @@ __global__ __launch_bounds__(THREADS) void paged_decode_kernel(const AttnParams 
                 s[n][h] = f32x4{0.f, 0.f, 0.f, 0.f};
                 if constexpr (!FOUR) {
 #pragma unroll
-                    for (int c = 0; c < DC; ++c) s[n][h] = Mfma16<T>::run(kreg[h][c], qf[n][c], s[n][h]);
+                    for (int c = 0; c < DC; ++c) s[n][h] = Mfma16<T>::run(x.k[h][c], qf[n][c], s[n][h]);
                 } else {
 #pragma unroll
                     for (int w = 0; w < kParts<T>; ++w)
 #pragma unroll
                         for (int c = 0; c < KC; ++c) {
-                            const i32x4 a = __builtin_bit_cast(i32x4, k4[h][c]);
+                            const i32x4 a = __builtin_bit_cast(i32x4, x.k4[h][c]);
                             // (Format 4: e2m1, its operand in the first four registers; 0: e4m3.)
                             s[n][h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
                                 __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1), q8[n][c][w], s[n][h], 4, 0, 0,
-                                static_cast<int>(k4s[h][c]), 0, qsc[n] - 4 * w);
+                                static_cast<int>(x.k4s[h][c]), 0, qsc[n] - 4 * w);
                         }
                 }
             }
-        // The K operands are consumed: the next tile's loads overlap the softmax and PV.
-        if (t + WAVES < t1) {
-            load_tile(t + WAVES, next);
-            if (t + 2 * WAVES < t1) next = entries(t + 2 * WAVES);
+        const int later = t + DEPTH * nslots;
+        if (later < nt) {
+            load_tile(x, later, e);
+            e = look_up(later + DEPTH * nslots);
         }
         v8 pf[NQ];
 #pragma unroll
@@ -385,74 +439,77 @@ __global__ __launch_bounds__(THREADS) void paged_decode_kernel(const AttnParams 
 #pragma unroll
             for (int n = 0; n < NQ; ++n) o[n][d] = Mfma16<T>::run(vf, pf[n], o[n][d]);
         }
+    };
+    while (t < nt) {
+#pragma unroll
+        for (int i = 0; i < DEPTH; ++i) {
+            if (t < nt) work(reg[i], next[i], t);
+            t += nslots;
+        }
     }
 
-    // The four wavefronts merge pairwise in LDS (the V tiles are done with): 2 and 3 hand their
-    // states to 0 and 1, then 1 to 0.
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) lsum[n] = sum4(lsum[n]);
+    // The wavefronts merge in LDS (the V tiles are done with), 16 rows at a time: every one leaves
+    // its state there and combines a share of the dims.
     float* const ex = reinterpret_cast<float*>(smem);
-    float* const st = ex + 2 * NQ * 16 * CP;
-#pragma unroll
-    for (int half = 2; half >= 1; half >>= 1) {
-        __syncthreads();
-        if (wave >= half && wave < 2 * half) {
-            const int slot = wave - half;
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) {
-#pragma unroll
-                for (int d = 0; d < DB; ++d)
-                    *reinterpret_cast<f32x4*>(ex + ((slot * NQ + n) * 16 + l16) * CP + 16 * d + 4 * g4) = o[n][d];
-                if (g4 == 0) *reinterpret_cast<f32x2*>(st + ((slot * NQ + n) * 16 + l16) * 2) = f32x2{m[n], lsum[n]};
-            }
-        }
-        __syncthreads();
-        if (wave < half) {
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) {
-                const f32x2 other = *reinterpret_cast<const f32x2*>(st + ((wave * NQ + n) * 16 + l16) * 2);
-                const float mn = fmaxf(m[n], other[0]);
-                const float wa = m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[n] - mn);
-                const float wb = other[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(other[0] - mn);
-                m[n] = mn;
-                lsum[n] = lsum[n] * wa + other[1] * wb;
-#pragma unroll
-                for (int d = 0; d < DB; ++d) {
-                    const f32x4 x = *reinterpret_cast<const f32x4*>(ex + ((wave * NQ + n) * 16 + l16) * CP + 16 * d + 4 * g4);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) o[n][d][i] = o[n][d][i] * wa + x[i] * wb;
-                }
-            }
-        }
-    }
-    if (wave != 0) return;
+    float* const st = ex + WAVES * 16 * CP;
+    constexpr int PER = DP / (4 * WAVES);  // dims of a lane: PER at PER (4 wave + g4) of row l16
+    typedef float fper __attribute__((ext_vector_type(PER % 4 == 0 ? 4 : 2)));
+    constexpr int VE = PER % 4 == 0 ? 4 : 2;
+    const int c0 = PER * (4 * wave + g4);
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
+        const float l = sum4(lsum[n]);
+        __syncthreads();
+#pragma unroll
+        for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4*>(ex + (wave * 16 + l16) * CP + 16 * d + 4 * g4) = o[n][d];
+        if (g4 == 0) *reinterpret_cast<f32x2*>(st + (wave * 16 + l16) * 2) = f32x2{m[n], l};
+        __syncthreads();
         if (!valid[n]) continue;
-        const float inv = lsum[n] > 0.f ? 1.f / lsum[n] : 0.f;
-        const int64_t tok = sp.q0 + pos[n];
-        if (alone) {
-            T* dst = static_cast<T*>(p.out) + head[n] * p.os[1] + tok * p.os[2];
-            typedef T t4 __attribute__((ext_vector_type(4)));
+        f32x2 state[WAVES];
+        float top = -INFINITY;
 #pragma unroll
-            for (int d = 0; d < DB; ++d) {
-                const int col = 16 * d + 4 * g4;
-                if (col >= p.dv) continue;
-                t4 w;
+        for (int w = 0; w < WAVES; ++w) {
+            state[w] = *reinterpret_cast<const f32x2*>(st + (w * 16 + l16) * 2);
+            top = fmaxf(top, state[w][0]);
+        }
+        float total = 0.f, acc[PER];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = from_f32<T>(o[n][d][i] * inv);
-                *reinterpret_cast<t4*>(dst + col) = w;
+        for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            const float wt = state[w][0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(state[w][0] - top);
+            total += wt * state[w][1];
+#pragma unroll
+            for (int i = 0; i < PER; i += VE) {
+                const fper x = *reinterpret_cast<const fper*>(ex + (w * 16 + l16) * CP + c0 + i);
+#pragma unroll
+                for (int e = 0; e < VE; ++e) acc[i + e] += wt * x[e];
             }
-            if (p.lse && g4 == 0)
-                p.lse[head[n] * p.ls[1] + tok * p.ls[2]] = lsum[n] > 0.f ? (m[n] + log2f(lsum[n])) * kLn2f : -INFINITY;
+        }
+        const float inv = total > 0.f ? 1.f / total : 0.f;
+        const int64_t tok = sp.q0 + pos[n];
+        if (p.splits == 1) {
+            T* dst = static_cast<T*>(p.out) + head[n] * p.os[1] + tok * p.os[2] + c0;
+            typedef T tper __attribute__((ext_vector_type(VE)));
+#pragma unroll
+            for (int i = 0; i < PER; i += VE) {
+                tper y;
+#pragma unroll
+                for (int e = 0; e < VE; ++e) y[e] = from_f32<T>(acc[i + e] * inv);
+                if (c0 + i < p.dv) *reinterpret_cast<tper*>(dst + i) = y;
+            }
+            if (p.lse && wave == 0 && g4 == 0)
+                p.lse[head[n] * p.ls[1] + tok * p.ls[2]] = total > 0.f ? (top + log2f(total)) * kLn2f : -INFINITY;
         } else {
             const int64_t at = (static_cast<int64_t>(split) * p.rows_total + tok) * p.hq + head[n];
 #pragma unroll
-            for (int d = 0; d < DB; ++d) {
-                const int col = 16 * d + 4 * g4;
-                if (col < p.dv) *reinterpret_cast<f32x4*>(p.part_o + at * DP + col) = o[n][d] * inv;
+            for (int i = 0; i < PER; i += VE) {
+                fper y;
+#pragma unroll
+                for (int e = 0; e < VE; ++e) y[e] = acc[i + e] * inv;
+                if (c0 + i < p.dv) *reinterpret_cast<fper*>(p.part_o + at * DP + c0 + i) = y;
             }
-            if (g4 == 0) p.part_lse[at] = lsum[n] > 0.f ? m[n] + log2f(lsum[n]) : -INFINITY;
+            if (wave == 0 && g4 == 0) p.part_lse[at] = total > 0.f ? top + log2f(total) : -INFINITY;
         }
     }
 }

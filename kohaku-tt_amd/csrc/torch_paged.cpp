@@ -4,6 +4,7 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/autograd.h>
 #include <torch/library.h>
 
 #include <cmath>
@@ -101,7 +102,7 @@ std::tuple<Tensor, Tensor> rotary(const Tensor& x_in, const optional<Tensor>& se
     const Tensor freq = inv_freq.contiguous();
     kmi_rotary_args a{};
     rotary_slot(a, 0, x, y);
-    Tensor k, ky = at::empty({0}, x.options());
+    Tensor k, ky;  // (undefined without a second tensor)
     if (given(second)) {
         k = unit_rows(*second);
         ky = at::empty_like(k);
@@ -125,6 +126,62 @@ std::tuple<Tensor, Tensor> rotary(const Tensor& x_in, const optional<Tensor>& se
     a.scale = scale;
     check(kmi_rotary(&a, stream_of(x)), "kmi_rotary");
     return {y, ky};
+}
+
+using RotaryOp = std::tuple<Tensor, Tensor>(const Tensor&, const optional<Tensor>&, const Tensor&, const Tensor&, bool,
+                                            double, bool);
+
+// The op through the dispatcher: the gradient's own gradient is the rotation again.
+const c10::TypedOperatorHandle<RotaryOp>& rotary_op() {
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("ktt::_rotary", "").typed<RotaryOp>();
+    return op;
+}
+
+// Rotary positions with gradients: the rotation back of whichever gradients there are.
+struct RotaryFn : public torch::autograd::Function<RotaryFn> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x,
+                                                  const optional<Tensor>& second, const Tensor& positions,
+                                                  const Tensor& inv_freq, bool interleaved, double scale, bool inverse) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        ctx->save_for_backward({positions, inv_freq});
+        ctx->saved_data["interleaved"] = interleaved;
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["inverse"] = inverse;
+        ctx->set_materialize_grads(false);
+        auto [y, ky] = rotary_op().call(x, second, positions, inv_freq, interleaved, scale, inverse);
+        if (!ky.defined()) return {y};
+        return {y, ky};
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                   torch::autograd::variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const Tensor first = grads[0], second = grads.size() > 1 ? grads[1] : Tensor();
+        Tensor gx, gk;
+        if (first.defined() || second.defined()) {
+            const bool both = first.defined() && second.defined();
+            auto [a, b] = rotary_op().call(first.defined() ? first : second, both ? optional<Tensor>(second) : std::nullopt,
+                                           saved[0], saved[1], ctx->saved_data["interleaved"].toBool(),
+                                           ctx->saved_data["scale"].toDouble(), !ctx->saved_data["inverse"].toBool());
+            (first.defined() ? gx : gk) = a;
+            if (both) gk = b;
+        }
+        return {gx, gk, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+// ktt::_rotary at AutogradCUDA.
+std::tuple<Tensor, Tensor> rotary_autograd(const Tensor& x, const optional<Tensor>& second, const Tensor& positions,
+                                           const Tensor& inv_freq, bool interleaved, double scale, bool inverse) {
+    if (at::GradMode::is_enabled() && (x.requires_grad() || (given(second) && second->requires_grad()))) {
+        auto out = RotaryFn::apply(x, second, positions, inv_freq, interleaved, scale, inverse);
+        return {out[0], out.size() > 1 ? out[1] : Tensor()};
+    }
+    at::AutoDispatchBelowADInplaceOrView below;
+    // (Traced tensors have no data: the dispatcher finds them their shapes.)
+    constexpr c10::DispatchKeySet traced({c10::DispatchKey::Python, c10::DispatchKey::PythonTLSSnapshot,
+                                          c10::DispatchKey::Functionalize});
+    if (!(x.key_set() & traced).empty()) return rotary_op().call(x, second, positions, inv_freq, interleaved, scale, inverse);
+    return rotary(x, second, positions, inv_freq, interleaved, scale, inverse);
 }
 
 // ---------------------------------------------------------------- the cache
@@ -364,4 +421,8 @@ TORCH_LIBRARY_IMPL(ktt, CUDA, m) {
     m.impl("_paged_append", TORCH_FN(kta::paged_append));
     m.impl("_paged_read", TORCH_FN(kta::paged_read));
     m.impl("_sdpa_paged", TORCH_FN(kta::sdpa_paged));
+}
+
+TORCH_LIBRARY_IMPL(ktt, AutogradCUDA, m) {
+    m.impl("_rotary", TORCH_FN(kta::rotary_autograd));
 }

@@ -35,6 +35,12 @@ import math
 
 import torch
 
+# (The overloads themselves: a call through the packet resolves them each time.)
+_ROTARY = torch.ops.ktt._rotary.default
+_APPEND = torch.ops.ktt._paged_append.default
+_READ = torch.ops.ktt._paged_read.default
+_SDPA = torch.ops.ktt._sdpa_paged.default
+
 __all__ = ["rotary", "rotary_frequencies", "paged_cache", "paged_append", "paged_read", "sdpa_paged"]
 
 
@@ -123,28 +129,8 @@ def rotary(x, positions, inv_freq, k=None, interleaved=False, scale=1.0):
     Returns the rotated tensor, in x's memory layout; with `k` (another tensor of the same
     tokens, any number of heads) both, from one launch.  Differentiable in x and k (the
     gradient is the rotation back)."""
-    y, ky = torch.ops.ktt._rotary(x, k, positions, inv_freq, interleaved, scale)
+    y, ky = _ROTARY(x, k, positions, inv_freq, interleaved, scale)
     return y if k is None else (y, ky)
-
-
-def _rotary_setup(ctx, inputs, output):
-    _x, second, positions, inv_freq, interleaved, scale, inverse = inputs
-    ctx.save_for_backward(positions, inv_freq)
-    ctx.args = (second is not None, interleaved, scale, inverse)
-    ctx.set_materialize_grads(False)
-
-
-def _rotary_backward(ctx, grad, grad_second):
-    positions, inv_freq = ctx.saved_tensors
-    has_second, interleaved, scale, inverse = ctx.args
-    if not has_second:
-        grad_second = None
-    gx = gk = None
-    if grad is not None or grad_second is not None:
-        first, second = (grad, grad_second) if grad is not None else (grad_second, None)
-        first, second = torch.ops.ktt._rotary(first, second, positions, inv_freq, interleaved, scale, not inverse)
-        gx, gk = (first, second if grad_second is not None else None) if grad is not None else (None, first)
-    return gx, gk, None, None, None, None, None
 
 
 # ---------------------------------------------------------------- the cache
@@ -182,8 +168,8 @@ def paged_append(k, v, k_cache, v_cache, block_table, key_lengths, cu_seq=None, 
     launch.  A 4-bit cache (`k_scale`, `v_scale`) is quantised on the way.  Tokens behind the
     last sequence write nothing; their rows of the rotated q are zero.  Returns the rotated q, or
     None without q.  Takes no gradients."""
-    return torch.ops.ktt._paged_append(k, v, k_cache, v_cache, block_table, key_lengths, cu_seq, q, inv_freq,
-                                       interleaved, rotary_scale, k_scale, v_scale)
+    return _APPEND(k, v, k_cache, v_cache, block_table, key_lengths, cu_seq, q, inv_freq,
+                   interleaved, rotary_scale, k_scale, v_scale)
 
 
 def paged_read(k_cache, v_cache, block_table, key_lengths, max_k, dtype=None, k_scale=None, v_scale=None):
@@ -192,7 +178,7 @@ def paged_read(k_cache, v_cache, block_table, key_lengths, max_k, dtype=None, k_
     given)."""
     if dtype is None:
         dtype = torch.bfloat16 if k_scale is not None else k_cache.dtype
-    return torch.ops.ktt._paged_read(k_cache, v_cache, block_table, key_lengths, max_k, dtype, k_scale, v_scale)
+    return _READ(k_cache, v_cache, block_table, key_lengths, max_k, dtype, k_scale, v_scale)
 
 
 def sdpa_paged(q, k_cache, v_cache, block_table, key_lengths, cu_seq_q=None, max_q=None, max_k=None, is_causal=True,
@@ -208,10 +194,39 @@ def sdpa_paged(q, k_cache, v_cache, block_table, key_lengths, cu_seq_q=None, max
     rows past it hold unspecified values.  `max_k` bounds the keys: those past it are not read
     (by default every key that `block_table` can name, which sizes a launch for that many, so
     give the batch's longest length where it is known).  No gradient."""
-    return torch.ops.ktt._sdpa_paged(q, k_cache, v_cache, block_table, key_lengths, cu_seq_q, max_q, max_k, is_causal,
-                                     scale, False, k_scale, v_scale)[0]
+    return _SDPA(q, k_cache, v_cache, block_table, key_lengths, cu_seq_q, max_q, max_k, is_causal,
+                 scale, False, k_scale, v_scale)[0]
+
+
+# ---------------------------------------------------------------- tracing
+
+
+def _rotary_shapes(x, second, positions, inv_freq, interleaved=False, scale=1.0, inverse=False):
+    return torch.empty_like(x), None if second is None else torch.empty_like(second)
+
+
+def _append_shapes(k, v, k_cache, v_cache, block_table, key_lengths, cu_seq=None, q=None, inv_freq=None,
+                   interleaved=False, rotary_scale=1.0, k_scale=None, v_scale=None):
+    return None if q is None else q.new_empty(q.shape)
+
+
+def _read_shapes(k_cache, v_cache, block_table, key_lengths, max_k, dtype, k_scale=None, v_scale=None):
+    wide = 1 if k_scale is None else 2
+    return tuple(
+        t.new_empty((block_table.size(0), t.size(1), max_k, wide * t.size(3)), dtype=dtype) for t in (k_cache, v_cache)
+    )
+
+
+def _sdpa_shapes(q, k_cache, v_cache, block_table, key_lengths, cu_seq_q=None, max_q=None, max_k=None, is_causal=True,
+                 scale=None, stats=False, k_scale=None, v_scale=None):
+    wide = 1 if v_scale is None else 2
+    out = q.new_empty((q.size(0), q.size(1), wide * v_cache.size(3)))
+    return out, q.new_empty((q.size(1) if stats else 0, q.size(0)), dtype=torch.float32)
 
 
 def install() -> None:
-    """Registers the rotation's gradient."""
-    torch.library.register_autograd("ktt::_rotary", _rotary_backward, setup_context=_rotary_setup)
+    """Registers the shapes of the ops' results, for tracing (``torch.compile``)."""
+    torch.library.register_fake("ktt::_rotary", _rotary_shapes)
+    torch.library.register_fake("ktt::_paged_append", _append_shapes)
+    torch.library.register_fake("ktt::_paged_read", _read_shapes)
+    torch.library.register_fake("ktt::_sdpa_paged", _sdpa_shapes)

@@ -466,6 +466,29 @@ def test_default_bounds_and_a_wide_table(ops, dev, bits):
     _check_attention(cut, None, c, q, None, False, 0.125, bits == 4, BF)
 
 
+@pytest.mark.parametrize("bits", [16, 4])
+def test_no_keys_at_all(ops, dev, bits):
+    """max_k of zero, a table of no pages, lengths of zero: zeros, and log-sum-exps of minus infinity."""
+    c = P.Cache([40, 7], 2, 64, 64, 16, BF, bits)
+    held = c.to(dev)
+    q = torch.randn(80, 8, 64, dtype=BF, device=dev)
+    cu = torch.tensor([0, 40, 80], dtype=torch.int32, device=dev)
+    none = {**held, "block_table": held["block_table"][:, :0]}
+    zero = {**held, "key_lengths": torch.zeros_like(held["key_lengths"])}
+    for kw in ({**held, "max_k": 0}, none, zero):
+        for qq, at in ((q[:2], {}), (q, {"cu_seq_q": cu, "max_q": 40})):
+            out = ops.sdpa_paged(qq, **kw, **at)
+            assert bool((out == 0).all())
+    k, v = (torch.zeros(2, 2, 64, dtype=BF, device=dev) for _ in "kv")
+    before = {n: t.clone() for n, t in held.items()}
+    ops.paged_append(k, v, **none)
+    ops.paged_append(k, v, **zero)
+    assert all(torch.equal(before[n].view(torch.uint8), held[n].view(torch.uint8)) for n in held)
+    kd, vd = ops.paged_read(none["k_cache"], none["v_cache"], none["block_table"], none["key_lengths"], 20,
+                            k_scale=held.get("k_scale"), v_scale=held.get("v_scale"))
+    assert bool((kd == 0).all()) and bool((vd == 0).all())
+
+
 # ---------------------------------------------------------------- together
 
 

@@ -282,3 +282,29 @@ def test_plain_attention_is_torchs():
     assert bool((size >= out.abs() - 1e-12).all())
     none, _, _, _ = P.attention(q, k[:3], v[:3], True, 0.2)
     assert bool((none[:2] == 0).all())
+
+
+def test_traced_calls_know_their_shapes():
+    """Fake CUDA tensors trace through the ops without a launch (no GPU is there)."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        x = torch.empty(2, 10, 4, 64, dtype=torch.bfloat16, device="cuda").transpose(1, 2)
+        k = torch.empty(2, 10, 2, 64, dtype=torch.bfloat16, device="cuda").transpose(1, 2)
+        pos, freq = torch.empty(10, dtype=torch.int64, device="cuda"), torch.empty(16, device="cuda")
+        y, ky = kohakutt_amd.rotary(x, pos, freq, k=k)
+        assert y.stride() == x.stride() and ky.shape == k.shape
+        assert kohakutt_amd.rotary(x, pos, freq).shape == x.shape
+        z = kohakutt_amd.rotary(x.detach().requires_grad_(), pos, freq)
+        assert z.requires_grad and z.shape == x.shape
+        for bits in (16, 4):
+            held = kohakutt_amd.paged_cache(5, 2, 16, 64, head_dim_v=96, bits=bits)
+            table, lens = torch.empty(3, 2, dtype=torch.int32, device="cuda"), torch.empty(3, dtype=torch.int32, device="cuda")
+            q, kk, v = (torch.empty(3, n, d, dtype=torch.bfloat16, device="cuda") for n, d in ((4, 64), (2, 64), (2, 96)))
+            assert kohakutt_amd.paged_append(kk, v, **held, block_table=table, key_lengths=lens) is None
+            got = kohakutt_amd.paged_append(kk, v, **held, block_table=table, key_lengths=lens, q=q, inv_freq=freq)
+            assert got.shape == q.shape
+            rk, rv = kohakutt_amd.paged_read(**held, block_table=table, key_lengths=lens, max_k=20)
+            assert rk.shape == (3, 2, 20, 64) and rv.shape == (3, 2, 20, 96) and rk.dtype == torch.bfloat16
+            out = kohakutt_amd.sdpa_paged(q, **held, block_table=table, key_lengths=lens)
+            assert out.shape == (3, 4, 96) and out.dtype == torch.bfloat16
