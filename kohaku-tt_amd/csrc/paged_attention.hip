@@ -72,12 +72,17 @@ Plan make_plan(const kmi_paged_attn_args* a) {
         pl.rows = vrows <= 16 ? 16 : 32;
         pl.nx = 1;
         // Two workgroups of four wavefronts per CU, a tile for each of a split's wavefronts and
-        // two where there are many splits (us at 4, 7 / 20, 40 splits: 14/2 heads x 777 keys x 64
-        // 8.1, 6.6; 4 bits, 3 x 4 tokens over 5001 keys 11.7, 12.3; 64 sequences x 2 heads x 8192
-        // keys x 128, at 2, 4, 6, 8 splits 100, 101, 103, 103, in 4 bits 52.5, 39.1, 38.9, 44.4).
+        // two where there are many splits (us in a graph at 4, 7 / 20, 40 splits: 14/2 heads x 777
+        // keys x 64 8.1, 6.6; 4 bits, 3 x 4 tokens over 5001 keys 11.7, 12.3; 64 sequences x 2
+        // heads x 8192 keys x 128, at 2, 4, 6, 8 splits 100, 101, 103, 103, in 4 bits 52.5, 39.1,
+        // 38.9, 44.4).
         pl.min_split = kDecodeTile;
         splits = std::min(ceil_div(512, std::max<int64_t>(1, units)),
                           std::max(std::min<int64_t>(ceil_div(keys, 4 * kDecodeTile), 8), keys / (8 * kDecodeTile)));
+        // Splits cost a second launch, 2.7 us of the GPU and 3 of the host; seven tiles a
+        // wavefront at head dim 64, the time of three and a half at 128, cost less in one (777
+        // keys as above: 7.3 us in a graph, but 8 against 11 from the host).
+        if (ceil_div(keys, 4 * kDecodeTile) * pl.dp <= 7 * 64) splits = 1;
     } else {
         const int64_t w4 = ceil_div(vrows, 128) * units;
         pl.row_groups = pl.dp <= 128 && w4 >= 448 ? 4 : 2;

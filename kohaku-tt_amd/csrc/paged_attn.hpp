@@ -20,15 +20,20 @@ struct AttnParams : fwd::AttnParams {
         const int per = fwd::fdiv(lk + splits - 1, fd_splits);
         return max((max(per, min_split) + unit - 1) / unit * unit, unit);
     }
+    // The table entry of a key of a sequence and its row there (uniform; not yet clamp_page'd, so
+    // that nothing waits for it before it is used).
+    __device__ __forceinline__ int entry_at(int seq, int key, int& row) const {
+        const int i = fwd::fdiv(key, c.fd_page);
+        row = key - i * c.page;
+        return uniform_i32(c.table + seq * c.table_stride + i);
+    }
     // The page of a key of a sequence and its row there (uniform).
     __device__ __forceinline__ int page_at(int seq, int key, int& row) const {
         if (head_pages) {
             row = key;
             return seq;
         }
-        const int i = fwd::fdiv(key, c.fd_page);
-        row = key - i * c.page;
-        return clamp_page(uniform_i32(c.table + seq * c.table_stride + i), c.pages);
+        return clamp_page(entry_at(seq, key, row), c.pages);
     }
     __device__ __forceinline__ const char* k_rows(int seq, int kvh, int key) const {
         int row;

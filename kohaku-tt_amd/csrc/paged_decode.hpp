@@ -1,14 +1,17 @@
 // Attention over a paged cache for few query rows: single tokens and short drafts, at most 32
 // "virtual rows" (query tokens x GQA group) per (sequence, K/V head).
 //
-// Bound by the cache's bytes.  A unit's keys are split over workgroups and dealt to their four
-// wavefronts in tiles of 32, each tile two halves of 16 rows that lie in one page each (page
-// sizes are multiples of 16), read through a buffer resource of their own: rows past the last key
-// read as zeros, so nothing stale in a page is ever touched.  The wavefronts share nothing until
-// the end and so need no barrier: K goes straight into MFMA operand registers, V through a
-// private LDS tile read transposed; the next tile's loads and the table entries of the one after
-// are in flight during a tile's arithmetic.  S^T = K Q^T leaves a query row per lane, its
-// softmax state is scalar; P feeds O^T += V^T P^T as it stands.
+// Bound by the cache's bytes.  A unit's keys are dealt in tiles of 32 to the wavefronts of its
+// splits in turn.  Each tile is two halves of 16 rows (page sizes are multiples of 16), read through
+// a buffer resource that ends with the sequence: rows past the last key read as zeros, so nothing
+// stale in a page is ever touched.  The wavefronts share nothing until the end and so need no
+// barrier: K goes straight into MFMA operand registers, V through a private LDS tile read
+// transposed; the next tile's loads and the table entries of the one after are in flight during a
+// tile's softmax and PV.  S^T = K Q^T leaves a query row per lane, its softmax state is scalar; P
+// feeds O^T += V^T P^T as it stands, in two 16-bit parts (a second product, hidden behind the
+// loads: 64 sequences x 2 heads x 8192 keys x 128 100.2 against 100.4 us, in 4 bits 35.5 against
+// 35.1), so that results are as close to 64-bit ones as their own rounding (0.0017 relative where
+// one part gave 0.0023).
 //
 // 16-bit caches: 16x16x32 MFMAs.  4-bit caches: the codes of K are the operand of the scaled
 // 16x16x128 MFMA as they lie in memory, with the cache's own scale bytes; no key is ever
@@ -16,6 +19,14 @@
 // significant bits, 2^-4 apart, on one power of two per row: bf16's eight bits fit two parts
 // exactly (elements below 2^-13 of the row's largest to within 2^-17 of it), fp16's eleven fit
 // three.  V's codes are widened by the packed conversions on their way into the LDS tile.
+//
+// Measured in a graph: that 16-bit call reads at 5.36 TB/s (a copy moves 5.13, the dense decode
+// kernel 97 us), the 4-bit one (142 MB) at 4.0 and at 5.2 with four times the keys: 13 us of
+// start, first latencies and merge are fixed.  What made it so, in 4 bits: entries and lengths read
+// side by side, table entries clamped and scale bytes widened where they are used (a widening left
+// where the byte was loaded waited for the whole next tile: 38.4 -> 35.5 us), ranges computed and
+// keys hidden in a sequence's last tile alone.  Two or three tiles in flight were no faster (35.5,
+// 37.1), nor eight wavefronts a workgroup.
 #pragma once
 
 #include "paged_attn.hpp"
@@ -76,6 +87,7 @@ constexpr int THREADS = WAVES * kWave;
 constexpr int TK = 32;                // keys of a tile
 constexpr float kLazy = 8.f;          // log2 units a row max may grow before O is rescaled
 constexpr float kLn2f = 0.6931471805599453f;
+constexpr uint32_t kOpen = 0x7fffffffu;  // the range of a resource whose rows are all there
 constexpr uint32_t kNone = 0x80000000u;  // an offset past every range: reads as zeros
 
 // Parts of a 4-bit call's Q.
@@ -92,15 +104,18 @@ constexpr size_t decode_lds() {
     return v > merge ? v : merge;
 }
 
+// Wavefronts per SIMD the kernel is held to: four for 16 rows of a 4-bit cache, whose tiles are
+// small and which is bound by how many wavefronts work at once.
+constexpr int decode_occupancy(int dp, int nq, bool four) { return four && nq == 1 && dp <= 128 ? 4 : 1; }
+
 template <typename T, int DP, int NQ, bool FOUR>
-__global__ __launch_bounds__(THREADS) void paged_decode_kernel(const AttnParams p) {
+__global__ __launch_bounds__(THREADS, decode_occupancy(DP, NQ, FOUR)) void paged_decode_kernel(const AttnParams p) {
     typedef typename Mfma16<T>::v8 v8;
     constexpr int DC = DP / 32;                // K fragments of a key row (16 bits)
     constexpr int KC = (DP + 127) / 128;       // the same at 4 bits
     constexpr int DB = DP / 16;                // output blocks
     constexpr int VP = v_pitch(DP);
     constexpr int CP = DP + 4;
-    constexpr int DEPTH = FOUR ? 2 : 1;  // tiles of a wavefront in flight
     // V staging, 16 bits: VPS lanes a row (a power of two; those past the padded row idle).
     constexpr int NCH = DP / 8;
     constexpr int VPS = NCH <= 4 ? 4 : NCH <= 8 ? 8 : NCH <= 16 ? 16 : 32;
@@ -125,14 +140,14 @@ __global__ __launch_bounds__(THREADS) void paged_decode_kernel(const AttnParams 
     // first table entries are so known before the sequence's length, and read beside it.
     const int slot = split * WAVES + wave, nslots = p.splits * WAVES;
 
-    // Tiles in registers.
+    // A tile in registers.
     struct TileRegs {
         v8 k[FOUR ? 1 : 2][FOUR ? 1 : DC];
         u32x4 v[FOUR ? 1 : 2][FOUR ? 1 : KIT];
         u32x4 k4[FOUR ? 2 : 1][FOUR ? KC : 1], v4[FOUR ? 2 : 1][FOUR ? R4 : 1];
-        uint32_t k4s[FOUR ? 2 : 1][FOUR ? KC : 1], v4s[FOUR ? 2 : 1][FOUR ? R4 : 1];
+        uint8_t k4s[FOUR ? 2 : 1][FOUR ? KC : 1], v4s[FOUR ? 2 : 1][FOUR ? R4 : 1];
     };
-    TileRegs reg[DEPTH];
+    TileRegs x;
     T* const vl = reinterpret_cast<T*>(smem) + wave * TK * VP;
     const int krow = lane / VPS, dg = lane % VPS;
     const uint32_t kst = static_cast<uint32_t>(p.c.ks[2]), vst = static_cast<uint32_t>(p.c.vs[2]);
@@ -149,7 +164,7 @@ __global__ __launch_bounds__(THREADS) void paged_decode_kernel(const AttnParams 
     };
     auto entry = [&](int key) {
         Entry e;
-        e.page = p.page_at(seq, max(min(key, p.c.capacity - 1), 0), e.row);
+        e.page = p.entry_at(seq, max(min(key, p.c.capacity - 1), 0), e.row);
         return e;
     };
     // (Page strides are below 2^32 bytes.)
@@ -178,10 +193,21 @@ __global__ __launch_bounds__(THREADS) void paged_decode_kernel(const AttnParams 
             vsoff[i] = in ? r * vss + ch : kNone;
         }
     }
-    // Requests `rows` rows (at most 16 n) from an entry on into halves h .. h + n - 1.
-    auto request = [&](TileRegs& x, const Entry& e, int rows, int h0, int n) __attribute__((always_inline)) {
-        const auto rk = buffer_rsrc(at(kh, e, p.c.ks[0], kst), rows_extent(rows, kst, FOUR ? p.d / 2 : 2 * p.d));
-        const auto rv = buffer_rsrc(at(vh, e, p.c.vs[0], vst), rows_extent(rows, vst, FOUR ? p.dv / 2 : 2 * p.dv));
+    // Requests `rows` rows (16 n at most) from an entry on into halves h .. h + n - 1.
+    auto request = [&](Entry e, int rows, int h0, int n) __attribute__((always_inline)) {
+        e.page = clamp_page(e.page, p.c.pages);
+        // (Ranges matter at the sequence's end alone.)
+        uint32_t ek = kOpen, ev = kOpen, eks = kOpen, evs = kOpen;
+        if (rows < 16 * n) {
+            ek = rows_extent(rows, kst, FOUR ? p.d / 2 : 2 * p.d);
+            ev = rows_extent(rows, vst, FOUR ? p.dv / 2 : 2 * p.dv);
+            if (FOUR) {
+                eks = rows_extent(rows, kss, p.d / 32);
+                evs = rows_extent(rows, vss, p.dv / 32);
+            }
+        }
+        const auto rk = buffer_rsrc(at(kh, e, p.c.ks[0], kst), ek);
+        const auto rv = buffer_rsrc(at(vh, e, p.c.vs[0], vst), ev);
         if constexpr (!FOUR) {
 #pragma unroll
             for (int h = 0; h < n; ++h) {
@@ -192,8 +218,8 @@ __global__ __launch_bounds__(THREADS) void paged_decode_kernel(const AttnParams 
                 for (int i = 0; i < KIT; ++i) x.v[h0 + h][i] = buffer_load16(rv, voff[0] + (16 * h + i * RPP) * vst);
             }
         } else {
-            const auto rks = buffer_rsrc(at(ksh, e, p.c.kss[0], kss), rows_extent(rows, kss, p.d / 32));
-            const auto rvs = buffer_rsrc(at(vsh, e, p.c.vss[0], vss), rows_extent(rows, vss, p.dv / 32));
+            const auto rks = buffer_rsrc(at(ksh, e, p.c.kss[0], kss), eks);
+            const auto rvs = buffer_rsrc(at(vsh, e, p.c.vss[0], vss), evs);
 #pragma unroll
             for (int h = 0; h < n; ++h) {
 #pragma unroll
@@ -220,21 +246,19 @@ __global__ __launch_bounds__(THREADS) void paged_decode_kernel(const AttnParams 
         e.half[1] = whole ? e.half[0] : entry(TK * t + 16);
         return e;
     };
-    Entries next[DEPTH];  // of the tiles to request next
-#pragma unroll
-    for (int i = 0; i < DEPTH; ++i) next[i] = look_up(slot + i * nslots);
+    Entries next = look_up(slot);  // of the tile to request next
     const Span sp = p.span(seq);
     const int vrows = min(min(sp.lq, p.seq_q) * G, 16 * NQ);
     const int lk = sp.lk;
     if (vrows <= 0) return;  // (uniform)
     const int nt = (lk + TK - 1) / TK;
-    auto load_tile = [&](TileRegs& x, int t, const Entries& e) __attribute__((always_inline)) {
+    auto load_tile = [&](int t) __attribute__((always_inline)) {
         const int rows = lk - TK * t;
         if (whole) {
-            request(x, e.half[0], min(rows, TK), 0, 2);
+            request(next.half[0], rows, 0, 2);
         } else {
-            request(x, e.half[0], min(rows, 16), 0, 1);
-            request(x, e.half[1], min(rows - 16, 16), 1, 1);
+            request(next.half[0], rows, 0, 1);
+            request(next.half[1], rows - 16, 1, 1);
         }
     };
 
@@ -250,6 +274,7 @@ __global__ __launch_bounds__(THREADS) void paged_decode_kernel(const AttnParams 
         head[n] = kvh * G + (rr - pos[n] * G);
         lim[n] = p.causal ? min(lk, lk - sp.lq + pos[n] + 1) : lk;
     }
+    const int every = p.causal ? min(lk, lk - sp.lq + 1) : lk;  // keys below it are seen by every row
     // A negative scale flips Q's sign, so that the row maximum of the products is that of the
     // logits; a zero one becomes a factor that finite products vanish under.
     const float c2 = fmaxf(fabsf(p.scale_log2), 1e-30f);
@@ -315,17 +340,15 @@ __global__ __launch_bounds__(THREADS) void paged_decode_kernel(const AttnParams 
         }
     }
 
-    // The first tiles, and the entries of those behind them.
+    // The first tile, and the entries of the one behind it.
     int t = slot;
-#pragma unroll
-    for (int i = 0; i < DEPTH; ++i)
-        if (t + i * nslots < nt) {
-            load_tile(reg[i], t + i * nslots, next[i]);
-            next[i] = look_up(t + (i + DEPTH) * nslots);
-        }
+    if (t < nt) {
+        load_tile(t);
+        next = look_up(t + nslots);
+    }
 
     // The tile's V rows into the wavefront's LDS.
-    auto stage = [&](const TileRegs& x) __attribute__((always_inline)) {
+    auto stage = [&] {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             if constexpr (!FOUR) {
@@ -363,13 +386,11 @@ __global__ __launch_bounds__(THREADS) void paged_decode_kernel(const AttnParams 
         neg_m[n] = lsum[n] = 0.f;
     }
 
-    // A tile's products, softmax and PV; once its K operands are consumed, the tile DEPTH steps on
-    // is requested into its registers.
-    auto work = [&](TileRegs& x, Entries& e, int t) __attribute__((always_inline)) {
+    for (; t < nt; t += nslots) {
         // LDS keeps one wavefront's accesses in order (the previous tile's reads, these writes,
         // this tile's reads): only the compiler must keep it.
         __asm__ volatile("" ::: "memory");
-        stage(x);
+        stage();
         f32x4 s[NQ][2];
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
@@ -392,21 +413,24 @@ __global__ __launch_bounds__(THREADS) void paged_decode_kernel(const AttnParams 
                         }
                 }
             }
-        const int later = t + DEPTH * nslots;
-        if (later < nt) {
-            load_tile(x, later, e);
-            e = look_up(later + DEPTH * nslots);
+        // The K operands are consumed and V is in LDS: the next tile's loads overlap the softmax and
+        // PV.
+        if (t + nslots < nt) {
+            load_tile(t + nslots);
+            next = look_up(t + 2 * nslots);
         }
-        v8 pf[NQ];
+        v8 pf[NQ], rest[NQ];  // the weights' two parts
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
             // Lane (g4, l16), register i of half h: key 16 h + 4 g4 + i of row l16.
-            const int rel = lim[n] - TK * t - 4 * g4;
+            if (TK * t + TK > every) {
+                const int rel = lim[n] - TK * t - 4 * g4;
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (16 * h + i >= rel) s[n][h][i] = -INFINITY;
+                    for (int i = 0; i < 4; ++i)
+                        if (16 * h + i >= rel) s[n][h][i] = -INFINITY;
+            }
             float mx = fmaxf(fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][0][2], s[n][0][3])),
                              fmaxf(fmaxf(s[n][1][0], s[n][1][1]), fmaxf(s[n][1][2], s[n][1][3])));
             if (__builtin_amdgcn_ballot_w64(mx * c2 > thr[n])) {
@@ -429,6 +453,7 @@ __global__ __launch_bounds__(THREADS) void paged_decode_kernel(const AttnParams 
                     const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][h][i], c2, neg_m[n]));
                     lsum[n] += e;
                     pf[n][4 * h + i] = static_cast<T>(e);
+                    rest[n][4 * h + i] = static_cast<T>(e - static_cast<float>(pf[n][4 * h + i]));
                 }
         }
         const T* vsrc = vl + (4 * g4 + (l16 >> 2)) * VP + 4 * (l16 & 3);
@@ -437,14 +462,7 @@ __global__ __launch_bounds__(THREADS) void paged_decode_kernel(const AttnParams 
             const u32x2 lo = tr_read(vsrc + 16 * d), hi = tr_read(vsrc + 16 * VP + 16 * d);
             const v8 vf = __builtin_bit_cast(v8, u32x4{lo[0], lo[1], hi[0], hi[1]});
 #pragma unroll
-            for (int n = 0; n < NQ; ++n) o[n][d] = Mfma16<T>::run(vf, pf[n], o[n][d]);
-        }
-    };
-    while (t < nt) {
-#pragma unroll
-        for (int i = 0; i < DEPTH; ++i) {
-            if (t < nt) work(reg[i], next[i], t);
-            t += nslots;
+            for (int n = 0; n < NQ; ++n) o[n][d] = Mfma16<T>::run(vf, rest[n], Mfma16<T>::run(vf, pf[n], o[n][d]));
         }
     }
 

@@ -349,7 +349,7 @@ std::tuple<Tensor, Tensor> paged_read(const Tensor& k_cache, const Tensor& v_cac
     return {k, v};
 }
 
-// (out [T, H, Dv], lse [H, T] when `stats`, else empty.)
+// (out [T, H, Dv], lse [H, T] when `stats`, else none.)
 std::tuple<Tensor, Tensor> sdpa_paged(const Tensor& q_in, const Tensor& k_cache, const Tensor& v_cache,
                                       const Tensor& table, const Tensor& lengths, const optional<Tensor>& cu,
                                       optional<int64_t> max_q, optional<int64_t> max_k, bool is_causal,
@@ -378,16 +378,20 @@ std::tuple<Tensor, Tensor> sdpa_paged(const Tensor& q_in, const Tensor& k_cache,
     c10::DeviceGuard guard(q_in.device());
     const Tensor q = rows_operand(q_in);
     Tensor out = at::empty({c.tokens, q.size(1), c.head_dim_v}, q.options());
-    Tensor lse = at::empty({stats ? q.size(1) : 0, c.tokens}, q.options().dtype(at::kFloat));
+    Tensor lse;  // (undefined without statistics)
+    if (stats) lse = at::empty({q.size(1), c.tokens}, q.options().dtype(at::kFloat));
     if (c.tokens == 0) return {out, lse};
-    if (c.batch == 0) return {out.zero_(), lse.fill_(-INFINITY)};
+    if (c.batch == 0) {
+        if (stats) lse.fill_(-INFINITY);
+        return {out.zero_(), lse};
+    }
     a.q = q.data_ptr();
     a.out = out.data_ptr();
     if (stats) a.lse = lse.data_ptr<float>();
     for (int i = 0; i < 2; ++i) {
         a.q_stride[i] = q.stride(i);
         a.o_stride[i] = out.stride(i);
-        a.lse_stride[i] = lse.stride(i);
+        if (stats) a.lse_stride[i] = lse.stride(i);
     }
     a.heads_q = q.size(1);
     a.causal = is_causal;

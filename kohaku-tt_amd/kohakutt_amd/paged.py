@@ -221,7 +221,7 @@ def _sdpa_shapes(q, k_cache, v_cache, block_table, key_lengths, cu_seq_q=None, m
                  scale=None, stats=False, k_scale=None, v_scale=None):
     wide = 1 if v_scale is None else 2
     out = q.new_empty((q.size(0), q.size(1), wide * v_cache.size(3)))
-    return out, q.new_empty((q.size(1) if stats else 0, q.size(0)), dtype=torch.float32)
+    return out, q.new_empty((q.size(1), q.size(0)), dtype=torch.float32) if stats else None
 
 
 def install() -> None:
