@@ -153,16 +153,22 @@ __device__ __forceinline__ void attn_tile(const P& p, unsigned char* smem, const
     const char* const vbase = reinterpret_cast<const char*>(static_cast<const T*>(p.v) + vb + kvh * p.vs[1] +
                                                             static_cast<int64_t>(k0) * p.vs[2]);
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(smem));
+    const auto held = [&] {
+        if constexpr (PAGED)
+            return p.rows(seq, kvh);
+        else
+            return 0;
+    }();
     auto request_k = [&](int t, int buf) {
         if constexpr (PAGED)
-            TL::request_pieces([&](int key) { return p.k_rows(seq, kvh, s0 + min(key, lk - 1)); }, kst, t * KT, lk, p.d * ES,
+            TL::request_pieces([&](int key) { return held.k_rows(s0 + min(key, lk - 1)); }, kst, t * KT, lk, p.d * ES,
                                okk, wave, lds0 + buf * TILE_B);
         else
             TL::request(kbase, kst, t * KT, lk, p.d * ES, okk, wave, lds0 + buf * TILE_B);
     };
     auto request_v = [&](int t, int buf) {
         if constexpr (PAGED)
-            TL::request_pieces([&](int key) { return p.v_rows(seq, kvh, s0 + min(key, lk - 1)); }, vst, t * KT, lk, p.dv * ES,
+            TL::request_pieces([&](int key) { return held.v_rows(s0 + min(key, lk - 1)); }, vst, t * KT, lk, p.dv * ES,
                                ovv, wave, lds0 + (2 + buf) * TILE_B);
         else
             TL::request(vbase, vst, t * KT, lk, p.dv * ES, ovv, wave, lds0 + (2 + buf) * TILE_B);

@@ -84,13 +84,41 @@ Plan make_plan(const kmi_paged_attn_args* a) {
         // keys as above: 7.3 us in a graph, but 8 against 11 from the host).
         if (ceil_div(keys, 4 * kDecodeTile) * pl.dp <= 7 * 64) splits = 1;
     } else {
-        const int64_t w4 = ceil_div(vrows, 128) * units;
-        pl.row_groups = pl.dp <= 128 && w4 >= 448 ? 4 : 2;
+        // Row tiles of the call, from its tokens (a tile begun per unit counts half).
+        const auto tiles = [&](int64_t rows) {
+            return std::min(ceil_div(vrows, rows) * units,
+                            ceil_div(a->cache.tokens * G, rows) * a->cache.heads_kv + units / 2);
+        };
+        const int64_t t4 = tiles(128), t2 = std::max<int64_t>(1, tiles(64));
+        // 128-row workgroups where they fill the chip (two a CU; one past head dim 128, of 64
+        // rows).  Prompts from their start do not pay for a merge, so that they take 64 rows
+        // instead; over longer keys the splits fill it, of 128 rows unless those are few.
+        // Measured (us, 64 rows at 1, 2, 4, 8 splits / 128 rows at 1, 2, 4, 8):
+        //   4 x up to 1024 tokens of 32/8 heads over 8192 keys x 128 (744 tiles of 128) 384, 437,
+        //     472, 577 / 353, 385, 399, 482
+        //   8 ragged x 16/2 over up to 7000 x 128 (286) 111, 97, 114, 153 / 153, 98, 94, 119
+        //   2 x 777 of 16/8 over 4500 x 128, 4 bits (200) 90, 101, 106, 126 / 110, 90, 99, 111
+        //   512 of 16/2 over 16384 x 128 (64) 246, 134, 106, 110 / 340, 181, 107, 97
+        //   512 of 14/2 over 8192 x 64 (56) 84, 50, 37, 43 / 134, 75, 44, 35
+        //   8 x 16 of 16/2 over 4096 x 128 (16) 67, 41, 27, 22, at 16 24 / 91, 53, 34, 25
+        //   prompts: 2048 of 14/2 x 64 (224) 26, 39, 42, 42 / 38, 38, 39, 39; 2 x 700 of 16/2 x 128
+        //     (176) 20, 33, 33, 33 / 23, 36, 35, 35; 4 x 2048 of 32/8 x 128 231, 366, .. / 197, 323, ..
+        const bool own = a->causal && 2 * a->max_q > keys;
+        const int64_t slots = pl.dp <= 128 ? 512 : 256;
+        pl.row_groups = 2;
+        pl.min_split = 256;
+        splits = std::max<int64_t>(1, slots / 2 / t2);
+        if (pl.dp <= 128 && t4 >= 448) {
+            pl.row_groups = 4;
+            splits = 1;
+        } else if (own) {
+            splits = t2 >= slots / 4 ? 1 : slots / 2 / t2;
+        } else if (pl.dp <= 128 && t4 >= 48) {
+            pl.row_groups = 4;
+            splits = std::max<int64_t>(2, slots / t4);
+        }
         pl.rows = 32 * pl.row_groups;
         pl.nx = static_cast<int>(ceil_div(vrows, pl.rows));
-        pl.min_split = 512;
-        splits = ceil_div(512, std::max<int64_t>(1, pl.nx * units));
-        if (pl.nx * units >= 256) splits = 1;
     }
     if (splits_override() > 0) splits = splits_override();
     pl.splits = static_cast<int>(

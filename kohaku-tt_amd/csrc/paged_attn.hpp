@@ -12,6 +12,8 @@ constexpr int kMaxSplits = 64;
 struct AttnParams : fwd::AttnParams {
     Cache c;
     int min_split;     // the fewest keys of a split
+    // Tile kernel's order: row tiles of a group, groups of a unit, sequences longest first.
+    int tile_group, tile_groups, sorted, rows_first;
     int head_pages;    // 1: c.k / c.v are dense copies [batch, heads_kv, capacity, dim] (no table)
     __device__ __forceinline__ Span span(int seq) const { return span_of(c, seq); }
     // Keys of a split of a sequence with `lk` keys, a multiple of `unit`: the sequence in at most
@@ -27,23 +29,49 @@ struct AttnParams : fwd::AttnParams {
         row = key - i * c.page;
         return uniform_i32(c.table + seq * c.table_stride + i);
     }
-    // The page of a key of a sequence and its row there (uniform).
-    __device__ __forceinline__ int page_at(int seq, int key, int& row) const {
-        if (head_pages) {
-            row = key;
-            return seq;
+    // A unit's keys and values, for the tile kernel: where rows from a key on lie (uniform).  Page
+    // strides are below 2^32 bytes.
+    struct Rows {
+        const char* k;
+        const char* v;
+        const int32_t* table;  // null: a dense copy, one page a sequence
+        uint32_t k_page, v_page, k_row, v_row;
+        int seq, pages, page;
+        fwd::FastDiv fd_page;
+        __device__ __forceinline__ int page_at(int key, int& row) const {
+            if (!table) {
+                row = key;
+                return seq;
+            }
+            const int i = fwd::fdiv(key, fd_page);
+            row = key - i * page;
+            return clamp_page(uniform_i32(table + i), pages);
         }
-        return clamp_page(entry_at(seq, key, row), c.pages);
-    }
-    __device__ __forceinline__ const char* k_rows(int seq, int kvh, int key) const {
-        int row;
-        const int page = page_at(seq, key, row);
-        return c.k + page * c.ks[0] + kvh * c.ks[1] + row * c.ks[2];
-    }
-    __device__ __forceinline__ const char* v_rows(int seq, int kvh, int key) const {
-        int row;
-        const int page = page_at(seq, key, row);
-        return c.v + page * c.vs[0] + kvh * c.vs[1] + row * c.vs[2];
+        __device__ __forceinline__ const char* k_rows(int key) const {
+            int row;
+            const uint64_t at = static_cast<uint32_t>(page_at(key, row));
+            return k + at * k_page + static_cast<uint64_t>(static_cast<uint32_t>(row)) * k_row;
+        }
+        __device__ __forceinline__ const char* v_rows(int key) const {
+            int row;
+            const uint64_t at = static_cast<uint32_t>(page_at(key, row));
+            return v + at * v_page + static_cast<uint64_t>(static_cast<uint32_t>(row)) * v_row;
+        }
+    };
+    __device__ __forceinline__ Rows rows(int seq, int kvh) const {
+        // (A dense copy's sequences may lie further apart than a page stride says.)
+        const int64_t base = head_pages ? seq : 0;
+        return Rows{c.k + base * c.ks[0] + kvh * c.ks[1],
+                    c.v + base * c.vs[0] + kvh * c.vs[1],
+                    head_pages ? nullptr : c.table + seq * c.table_stride,
+                    head_pages ? 0u : static_cast<uint32_t>(c.ks[0]),
+                    head_pages ? 0u : static_cast<uint32_t>(c.vs[0]),
+                    static_cast<uint32_t>(c.ks[2]),
+                    static_cast<uint32_t>(c.vs[2]),
+                    seq,
+                    c.pages,
+                    c.page,
+                    c.fd_page};
     }
 };
 

@@ -5,6 +5,8 @@
 // with few row tiles splits the keys over workgroups (fp32 partials, merged by a second launch).
 #pragma once
 
+#include <cstdlib>
+
 #include "attention_tile.hpp"
 #include "paged_attn.hpp"
 
@@ -14,34 +16,46 @@ namespace fwd {
 template <>
 inline constexpr bool kPagedKeys<paged::AttnParams> = true;
 
-// Workgroups: row tiles heaviest first, the splits of a row tile next to each other.  From eight
-// units (sequence, K/V head) on, unit u's lie on XCD u % 8 (block b runs on XCD b % 8), so that its
-// keys stay in one L2, with each row of tiles' units rotated by the row (ragged sequences would
-// otherwise meet the same few units' work row after row).  One more workgroup zeroes the rows
-// behind the last sequence.
+// The sequence with the `nth` most keys (the lower index first among equals), found by every
+// wavefront for itself: a lane a sequence, up to 64 of them.
+__device__ __forceinline__ int sorted_sequence(const paged::AttnParams& p, int nth) {
+    const int lane = threadIdx.x & 63;
+    const int lk = lane < p.batch ? min(max(p.c.klen[lane], 0), p.c.capacity) : -1;
+    int before = 0;
+    for (int j = 0; j < p.batch; ++j) {
+        const int other = __builtin_amdgcn_readlane(lk, j);
+        before += other > lk || (other == lk && j < lane) ? 1 : 0;
+    }
+    const uint64_t found = __builtin_amdgcn_ballot_w64(lane < p.batch && before == nth);
+    return __builtin_amdgcn_readfirstlane(found ? __builtin_ctzll(found) : 0);
+}
+
+// Workgroup order.  Row tiles of a unit (sequence, K/V head) read the same keys, so `group` of them
+// lie on one XCD (block b runs on XCD b % 8) next to each other and share its L2; groups go round the
+// XCDs there and back, those with most keys first: the longest sequence's heads, then the next
+// one's; where a causal call's keys are mostly its own queries (prompts from their start) the last
+// row tiles of every unit, then those before them.  One more workgroup zeroes the rows behind the last sequence.
 template <typename T, int DP, int RG>
 __global__ __launch_bounds__(NTHREADS, tile_waves(DP)) void paged_attn_tile_kernel(const paged::AttnParams p) {
     constexpr size_t TILES = 4 * sizeof(T) * Tile<T, DP, tile_keys(DP, RG)>::ELEMS;
     __shared__ __align__(1024) unsigned char smem[TILES];
-    const int units = p.batch * p.hkv;
     const int lin = blockIdx.x;
     if (lin == static_cast<int>(gridDim.x) - 1) {
         paged::zero_tail<T>(p);
         return;
     }
-    int bh, row;  // row: row tile and split
-    if (p.xcd_map == 3) {
-        const int x = lin & 7, s = lin >> 3;
-        const int nxu = (units - x + 7) >> 3;
-        if (nxu <= 0) return;
-        row = s / nxu;
-        if (row >= p.nx * p.splits) return;
-        bh = x + 8 * ((s - row * nxu + row) % nxu);
-    } else {
-        row = fdiv(lin, p.fd_units);
-        bh = lin - row * units;
+    const int x = lin & 7, s = lin >> 3, per = p.tile_group * p.splits;
+    const int round = s / per, i = s - round * per;
+    const int g = 8 * round + (round & 1 ? 7 - x : x);
+    const int units = p.batch * p.hkv;
+    const int unit = p.rows_first ? g % units : g / p.tile_groups, xg = p.rows_first ? g / units : g - unit * p.tile_groups;
+    const int split = i / p.tile_group, xi = xg * p.tile_group + (i - split * p.tile_group);
+    if (unit >= units || xi >= p.nx) return;
+    int bh = unit;
+    if (p.sorted) {
+        const int nth = fdiv(unit, p.fd_hkv);
+        bh = sorted_sequence(p, nth) * p.hkv + (unit - nth * p.hkv);
     }
-    const int xi = fdiv(row, p.fd_splits), split = row - xi * p.splits;
     attn_tile<T, DP, MK_NONE, RG>(p, smem, bh, p.causal ? p.nx - 1 - xi : xi, split);
 }
 
@@ -53,8 +67,17 @@ template <typename T, int DP>
 hipError_t launch_tile(const AttnParams& p_in, int rg, hipStream_t stream) {
     AttnParams p = p_in;
     const int units = p.batch * p.hkv;
-    p.xcd_map = units >= 8 ? 3 : 0;
-    const dim3 grid(static_cast<unsigned>((p.xcd_map == 3 ? 8 * ((units + 7) / 8) : units) * p.nx * p.splits + 1));
+    // All row tiles of a unit (32 at most), fewer where that leaves less than 32 groups to deal
+    // (4x1024 tokens of 32/8 heads over 8192 keys x 128: groups of 8, 16, 32 tiles 387, 363, 345 us;
+    // 512 tokens of 14/2 heads over 8192 keys x 64, 4, 16, 32 tiles 47, 48, 70).
+    p.tile_group = 32;
+    while (p.tile_group > 1 && (p.tile_group >= 2 * p.nx || units * ((p.nx + p.tile_group - 1) / p.tile_group) < 32))
+        p.tile_group /= 2;
+    p.rows_first = p.causal && 2 * static_cast<int64_t>(p.seq_q) > p.c.capacity;
+    p.tile_groups = (p.nx + p.tile_group - 1) / p.tile_group;
+    p.sorted = p.batch > 1 && p.batch <= 64 && static_cast<int64_t>(units) * p.nx * p.splits > 256;
+    const int rounds = (units * p.tile_groups + 7) / 8;
+    const dim3 grid(static_cast<unsigned>(8 * rounds * p.tile_group * p.splits + 1));
     if constexpr (DP <= 128) {
         if (rg == 4) {
             hipLaunchKernelGGL((fwd::paged_attn_tile_kernel<T, DP, 4>), grid, dim3(fwd::NTHREADS), 0, stream, p);

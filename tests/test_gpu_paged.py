@@ -427,7 +427,7 @@ def _kernel(new, heads, group, d):
     return capi.paged_attn_kernel(a)
 
 
-@pytest.mark.parametrize("new,kernel", [([1] * 4, "decode16"), ([4], "decode32"), ([300] * 4, "tile64"), ([2000] * 32, "tile128")])
+@pytest.mark.parametrize("new,kernel", [([1] * 4, "decode16"), ([4], "decode32"), ([40], "tile64"), ([300] * 4, "tile128"), ([2000] * 32, "tile128")])
 def test_kernels_by_rows(native, new, kernel):
     assert _kernel(new, 2, 8, 128) == kernel
 
