@@ -102,7 +102,8 @@ Plan make_plan(const kmi_paged_attn_args* a) {
         //   512 of 14/2 over 8192 x 64 (56) 84, 50, 37, 43 / 134, 75, 44, 35
         //   8 x 16 of 16/2 over 4096 x 128 (16) 67, 41, 27, 22, at 16 24 / 91, 53, 34, 25
         //   prompts: 2048 of 14/2 x 64 (224) 26, 39, 42, 42 / 38, 38, 39, 39; 2 x 700 of 16/2 x 128
-        //     (176) 20, 33, 33, 33 / 23, 36, 35, 35; 4 x 2048 of 32/8 x 128 231, 366, .. / 197, 323, ..
+        //     (176) 20, 33, 33, 33 / 23, 36, 35, 35; 4 x 2048 of 32/8 x 128 231, 366, .. / 197, 323, ..;
+        //     512 of 14/2 x 64 (56 of 64 rows) 10.0 whole, 13.2 in two
         const bool own = a->causal && 2 * a->max_q > keys;
         const int64_t slots = pl.dp <= 128 ? 512 : 256;
         pl.row_groups = 2;
@@ -112,7 +113,7 @@ Plan make_plan(const kmi_paged_attn_args* a) {
             pl.row_groups = 4;
             splits = 1;
         } else if (own) {
-            splits = t2 >= slots / 4 ? 1 : slots / 2 / t2;
+            splits = t2 >= slots / 8 ? 1 : slots / 4 / t2;
         } else if (pl.dp <= 128 && t4 >= 48) {
             pl.row_groups = 4;
             splits = std::max<int64_t>(2, slots / t4);
