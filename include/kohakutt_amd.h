@@ -333,7 +333,8 @@ int kmi_rotary(const kmi_rotary_args* args, void* stream);
 
 /*
  * A paged key / value cache: `pages` pages of page_size rows (a multiple of 16) per K/V
- * head, element (page, head, row, dim) at page * s[0] + head * s[1] + row * s[2] + dim.
+ * head, element (page, head, row, dim) at page * s[0] + head * s[1] + row * s[2] + dim; page strides
+ * below 2^30, row strides at most 2^24.
  * Sequence b's key p is row p % page_size of page block_table[b * table_stride + p / page_size];
  * it holds keys [0, key_lengths[b]), the new tokens of the call being the last of them.
  *   bits 16: values of `dtype` (BF16 or F16), head dims multiples of 8 up to 256, strides
@@ -402,10 +403,11 @@ int kmi_paged_read(const kmi_paged_cache* cache, void* k_out, void* v_out, int64
  * Attention of packed queries over a paged cache: out = softmax(scale q k^T) v, query r of
  * sequence b seeing keys [0, key_lengths[b]), with causal the first key_lengths[b] - Lq_b +
  * r + 1 of them (bottom-right); a query that sees no key gets zeros and lse minus infinity,
- * as do rows of no sequence.  q [tokens, heads_q, head_dim], out [tokens, heads_q, head_dim_v]
- * (element strides of the token and head dims, as kmi_attn_fwd's), lse optional fp32 natural log
- * [heads_q, tokens] with strides (head, token).  max_q covers every sequence's new tokens;
- * max_k sizes the launch (keys past it are still read).  Workspace:
+ * as do rows behind the last sequence (a call without sequences writes nothing).  q [tokens,
+ * heads_q, head_dim], out [tokens, heads_q, head_dim_v] (element strides of the token and head
+ * dims, as kmi_attn_fwd's), lse optional fp32 natural log [heads_q, tokens] with strides (head,
+ * token).  max_q covers every sequence's new tokens (rows of a sequence past it are not computed), max_k bounds the keys that are read and so the
+ * launch and, for a 4-bit cache with more than 32 rows per K/V head, the workspace.  Workspace:
  * kmi_paged_attn_workspace_bytes, 16-byte aligned, contents free before and after.
  */
 typedef struct kmi_paged_attn_args {

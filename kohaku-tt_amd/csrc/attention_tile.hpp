@@ -523,9 +523,11 @@ __device__ __forceinline__ void attn_tile(const P& p, unsigned char* smem, const
         if (kp == 1) return;
         const f32x4 st = ex[DB * 4 * kWave + lane];
         const float mn = fmaxf(m, st[0]);
-        // (Minus infinity: that wavefront's sums are zero.)
-        const float wa = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-        const float wb = st[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st[0] - mn);
+        // (Minus infinity: that wavefront's sums are zero, or NaN where its logits all were, which
+        // a merge of splits is to see.)
+        const auto none = [](float top, float sum) { return top == -INFINITY && (!PAGED || __float_as_uint(sum) == 0u); };
+        const float wa = none(m, lsum) ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+        const float wb = none(st[0], st[1]) ? 0.f : __builtin_amdgcn_exp2f(st[0] - mn);
         m = mn;
         lsum = lsum * wa + st[1] * wb;
 #pragma unroll
@@ -555,7 +557,8 @@ __device__ __forceinline__ void attn_tile(const P& p, unsigned char* smem, const
                         *reinterpret_cast<f32x4*>(p.part_o + at * DP + d) =
                             f32x4{o[b][4 * q] * inv, o[b][4 * q + 1] * inv, o[b][4 * q + 2] * inv, o[b][4 * q + 3] * inv};
                 }
-            if (h2 == 0) p.part_lse[at] = l > 0.f ? m + log2f(l) : -INFINITY;
+            // (By its bits: a NaN must reach the merge.)
+            if (h2 == 0) p.part_lse[at] = __float_as_uint(l) == 0u ? -INFINITY : m + log2f(l);
             return;
         }
     }

@@ -172,7 +172,7 @@ __global__ __launch_bounds__(MERGE_ROWS * kWave) void merge_kernel(const AttnPar
     }
     const int tok = static_cast<int>(row / p.hq), head = static_cast<int>(row - static_cast<int64_t>(tok) * p.hq);
     if (d0 < p.dv) {
-        const float inv = total > 0.f ? 1.f / total : 0.f;
+        const float inv = total == 0.f ? 0.f : 1.f / total;
         T y[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) y[e] = from_f32<T>(acc[e] * inv);
@@ -180,7 +180,7 @@ __global__ __launch_bounds__(MERGE_ROWS * kWave) void merge_kernel(const AttnPar
         __builtin_memcpy(__builtin_assume_aligned(dst, E * 2), y, E * 2);
     }
     if (p.lse && lane == 0)
-        p.lse[head * p.ls[1] + tok * p.ls[2]] = total > 0.f ? (top + log2f(total)) * 0.6931471805599453f : -INFINITY;
+        p.lse[head * p.ls[1] + tok * p.ls[2]] = total == 0.f ? -INFINITY : (top + log2f(total)) * 0.6931471805599453f;
 }
 
 template <typename T, int DP>
@@ -206,12 +206,20 @@ hipError_t run_dim(const AttnParams& p, const Plan& pl, bool four, hipStream_t s
     }
 }
 
-// Launches hold fewer than 2^32 threads; 32-bit workgroup arithmetic fits below that.
+// Workgroups that zero the rows behind the last sequence, should there be any: one per 64 KB of
+// output (none without offsets, where every row has a sequence).
+int tail_blocks(const kmi_paged_attn_args* a) {
+    if (!a->cache.cu_seqlens) return 0;
+    return static_cast<int>(std::min<int64_t>(512, ceil_div(a->cache.tokens * a->heads_q * a->cache.head_dim_v, 1 << 15)));
+}
+
+// Launches hold fewer than 2^32 threads (2^24 workgroups); the tile kernel's rounds its row tiles
+// of a unit up to groups of at most 32, fewer than twice as many.
 bool grid_fits(const kmi_paged_attn_args* a, const Plan& pl) {
     const double units = static_cast<double>(a->cache.batch) * a->cache.heads_kv;
     const double blocks = units * pl.nx * pl.splits;
     const double rows = static_cast<double>(a->cache.tokens) * a->heads_q;
-    return blocks < (1 << 23) - 1 && (pl.splits == 1 || rows < (1 << 26));
+    return blocks < (1 << 23) - (1 << 15) && (pl.splits == 1 || rows < (1 << 26));
 }
 
 }  // namespace
@@ -301,6 +309,7 @@ extern "C" int kmi_paged_attn(const kmi_paged_attn_args* a, void* workspace, siz
     p.splits = pl.splits;
     p.min_split = pl.min_split;
     p.nx = pl.nx;
+    p.tail_blocks = tail_blocks(a);
     p.rows_total = a->cache.tokens;
     p.fd_splits = fwd::fast_div(static_cast<uint32_t>(p.splits));
     p.fd_units = fwd::fast_div(static_cast<uint32_t>(p.batch * p.hkv));

@@ -14,6 +14,7 @@ struct AttnParams : fwd::AttnParams {
     int min_split;     // the fewest keys of a split
     // Tile kernel's order: row tiles of a group, groups of a unit, sequences longest first.
     int tile_group, tile_groups, sorted, rows_first;
+    int tail_blocks;   // workgroups that zero the rows behind the last sequence
     int head_pages;    // 1: c.k / c.v are dense copies [batch, heads_kv, capacity, dim] (no table)
     __device__ __forceinline__ Span span(int seq) const { return span_of(c, seq); }
     // Keys of a split of a sequence with `lk` keys, a multiple of `unit`: the sequence in at most
@@ -76,27 +77,28 @@ struct AttnParams : fwd::AttnParams {
 };
 
 // Zeros (and log-sum-exps of minus infinity) for the rows behind the last sequence, in a split
-// call through the merge: one workgroup of a call does it.
+// call through the merge, by the call's tail_blocks last workgroups.
 template <typename T>
-__device__ __forceinline__ void zero_tail(const AttnParams& p) {
-    if (!p.c.cu) return;
+__device__ __forceinline__ void zero_tail(const AttnParams& p, int block) {
     const int t0 = min(max(uniform_i32(p.c.cu + p.c.batch), 0), p.c.tokens);
     const int vec = p.dv / 4;
+    const int64_t first = static_cast<int64_t>(block) * blockDim.x + threadIdx.x;
+    const int64_t stride = static_cast<int64_t>(p.tail_blocks) * blockDim.x;
     const int64_t n = static_cast<int64_t>(p.c.tokens - t0) * p.hq;
     if (p.splits > 1) {
-        for (int64_t i = threadIdx.x; i < n * p.splits; i += blockDim.x) {
+        for (int64_t i = first; i < n * p.splits; i += stride) {
             const int64_t s = i / n;
             p.part_lse[(s * p.rows_total + t0) * p.hq + (i - s * n)] = -INFINITY;
         }
         return;
     }
     typedef T t4 __attribute__((ext_vector_type(4)));
-    for (int64_t i = threadIdx.x; i < n * vec; i += blockDim.x) {
+    for (int64_t i = first; i < n * vec; i += stride) {
         const int64_t r = i / vec, t = t0 + r / p.hq, h = r % p.hq;
         *reinterpret_cast<t4*>(static_cast<T*>(p.out) + t * p.os[2] + h * p.os[1] + 4 * (i - r * vec)) = t4{};
     }
     if (p.lse)
-        for (int64_t r = threadIdx.x; r < n; r += blockDim.x)
+        for (int64_t r = first; r < n; r += stride)
             p.lse[(t0 + r / p.hq) * p.ls[2] + (r % p.hq) * p.ls[1]] = -INFINITY;
 }
 

@@ -128,8 +128,8 @@ __global__ __launch_bounds__(THREADS, decode_occupancy(DP, NQ, FOUR)) void paged
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g4 = lane >> 4, l16 = lane & 15;
     const int units = p.batch * p.hkv;
-    if (static_cast<int>(blockIdx.x) == units * p.splits) {
-        zero_tail<T>(p);
+    if (static_cast<int>(blockIdx.x) >= units * p.splits) {
+        zero_tail<T>(p, blockIdx.x - units * p.splits);
         return;
     }
     const int bh = fwd::fdiv(static_cast<int>(blockIdx.x), p.fd_splits);
@@ -495,7 +495,8 @@ __global__ __launch_bounds__(THREADS, decode_occupancy(DP, NQ, FOUR)) void paged
         for (int i = 0; i < PER; ++i) acc[i] = 0.f;
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) {
-            const float wt = state[w][0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(state[w][0] - top);
+            // (By the sum, not the maximum: logits that are all NaN leave that at minus infinity.)
+            const float wt = state[w][1] == 0.f ? 0.f : __builtin_amdgcn_exp2f(state[w][0] - top);
             total += wt * state[w][1];
 #pragma unroll
             for (int i = 0; i < PER; i += VE) {
@@ -504,7 +505,8 @@ __global__ __launch_bounds__(THREADS, decode_occupancy(DP, NQ, FOUR)) void paged
                 for (int e = 0; e < VE; ++e) acc[i + e] += wt * x[e];
             }
         }
-        const float inv = total > 0.f ? 1.f / total : 0.f;
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+        const float log = total == 0.f ? -INFINITY : top + log2f(total);
         const int64_t tok = sp.q0 + pos[n];
         if (p.splits == 1) {
             T* dst = static_cast<T*>(p.out) + head[n] * p.os[1] + tok * p.os[2] + c0;
@@ -517,7 +519,7 @@ __global__ __launch_bounds__(THREADS, decode_occupancy(DP, NQ, FOUR)) void paged
                 if (c0 + i < p.dv) *reinterpret_cast<tper*>(dst + i) = y;
             }
             if (p.lse && wave == 0 && g4 == 0)
-                p.lse[head[n] * p.ls[1] + tok * p.ls[2]] = total > 0.f ? (top + log2f(total)) * kLn2f : -INFINITY;
+                p.lse[head[n] * p.ls[1] + tok * p.ls[2]] = log * kLn2f;
         } else {
             const int64_t at = (static_cast<int64_t>(split) * p.rows_total + tok) * p.hq + head[n];
 #pragma unroll
@@ -527,7 +529,7 @@ __global__ __launch_bounds__(THREADS, decode_occupancy(DP, NQ, FOUR)) void paged
                 for (int e = 0; e < VE; ++e) y[e] = acc[i + e] * inv;
                 if (c0 + i < p.dv) *reinterpret_cast<fper*>(p.part_o + at * DP + c0 + i) = y;
             }
-            if (wave == 0 && g4 == 0) p.part_lse[at] = total > 0.f ? top + log2f(total) : -INFINITY;
+            if (wave == 0 && g4 == 0) p.part_lse[at] = log;
         }
     }
 }
@@ -536,13 +538,13 @@ template <typename T, int DP, int NQ, bool FOUR>
 hipError_t launch_decode_as(const AttnParams& p, hipStream_t stream) {
     constexpr size_t lds = decode_lds<T, DP, NQ>();
     if constexpr (lds > 64 * 1024) {
-        static const hipError_t attr =
+        const hipError_t attr =
             hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_decode_kernel<T, DP, NQ, FOUR>),
                                 hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
         if (attr != hipSuccess) return attr;
     }
     hipLaunchKernelGGL((paged_decode_kernel<T, DP, NQ, FOUR>),
-                       dim3(static_cast<unsigned>(p.batch * p.hkv * p.splits + 1)), dim3(THREADS), lds, stream, p);
+                       dim3(static_cast<unsigned>(p.batch * p.hkv * p.splits + p.tail_blocks)), dim3(THREADS), lds, stream, p);
     return hipGetLastError();
 }
 

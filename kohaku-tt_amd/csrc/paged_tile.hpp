@@ -34,14 +34,15 @@ __device__ __forceinline__ int sorted_sequence(const paged::AttnParams& p, int n
 // lie on one XCD (block b runs on XCD b % 8) next to each other and share its L2; groups go round the
 // XCDs there and back, those with most keys first: the longest sequence's heads, then the next
 // one's; where a causal call's keys are mostly its own queries (prompts from their start) the last
-// row tiles of every unit, then those before them.  One more workgroup zeroes the rows behind the last sequence.
+// row tiles of every unit, then those before them.  The last workgroups zero the rows behind the last
+// sequence.
 template <typename T, int DP, int RG>
 __global__ __launch_bounds__(NTHREADS, tile_waves(DP)) void paged_attn_tile_kernel(const paged::AttnParams p) {
     constexpr size_t TILES = 4 * sizeof(T) * Tile<T, DP, tile_keys(DP, RG)>::ELEMS;
     __shared__ __align__(1024) unsigned char smem[TILES];
     const int lin = blockIdx.x;
-    if (lin == static_cast<int>(gridDim.x) - 1) {
-        paged::zero_tail<T>(p);
+    if (lin >= static_cast<int>(gridDim.x) - p.tail_blocks) {
+        paged::zero_tail<T>(p, gridDim.x - 1 - lin);
         return;
     }
     const int x = lin & 7, s = lin >> 3, per = p.tile_group * p.splits;
@@ -77,7 +78,7 @@ hipError_t launch_tile(const AttnParams& p_in, int rg, hipStream_t stream) {
     p.tile_groups = (p.nx + p.tile_group - 1) / p.tile_group;
     p.sorted = p.batch > 1 && p.batch <= 64 && static_cast<int64_t>(units) * p.nx * p.splits > 256;
     const int rounds = (units * p.tile_groups + 7) / 8;
-    const dim3 grid(static_cast<unsigned>(8 * rounds * p.tile_group * p.splits + 1));
+    const dim3 grid(static_cast<unsigned>(8 * rounds * p.tile_group * p.splits + p.tail_blocks));
     if constexpr (DP <= 128) {
         if (rg == 4) {
             hipLaunchKernelGGL((fwd::paged_attn_tile_kernel<T, DP, 4>), grid, dim3(fwd::NTHREADS), 0, stream, p);

@@ -447,6 +447,74 @@ def test_calls_repeat_bit_for_bit_and_sequences_are_independent(ops, dev, bits):
         assert torch.equal(one, two)
 
 
+@pytest.mark.parametrize("new,before", [([1, 1, 1], [900, 41, 300]), ([60, 3, 2], [100, 41, 700]), ([130, 8], [4, 900])])
+def test_many_rows_behind_the_last_sequence(ops, dev, new, before):
+    """More of them than one workgroup zeroes (64 KB of output each), whole calls and split ones."""
+    _attend(ops, dev, new, before, 2, 4, 128, 128, 32, BF, 16, tail=700)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("rows,kernel", [(1, "decode16"), (5, "decode32"), (40, "tile64")])
+@pytest.mark.parametrize("keys,at", [(48, 3), (700, 650), (9000, 100), (33, 32)])
+def test_a_nan_key_is_not_lost(ops, dev, bits, rows, kernel, keys, at):
+    """One key that is NaN: every query that sees it is NaN, in calls split over their keys too
+    (where the part that holds it has no maximum or sum), those before it are as ever."""
+    heads, group, d = 2, 4, 64
+    c = P.Cache([keys], heads, d, d, 16, BF, bits)
+    held = c.to(dev)
+    page, row = int(held["block_table"][0, at // 16]), at % 16
+    if bits == 16:
+        held["k_cache"][page, :, row] = math.nan
+    else:
+        held["k_scale"][page, :, row] = 255
+    q = _randn(rows, heads * group, d, seed=1, dtype=BF).to(dev)
+    cu = torch.tensor([0, rows], dtype=torch.int32, device=dev)
+    assert _kernel([rows], heads, group, d) == kernel
+    for causal in (True, False):
+        out = ops.sdpa_paged(q, **held, cu_seq_q=cu, max_q=rows, max_k=keys, is_causal=causal)
+        sees = torch.arange(rows) + keys - rows >= at if causal else torch.ones(rows, dtype=torch.bool)
+        assert torch.equal(out.isnan().all(-1).all(-1).cpu(), sees)
+        assert torch.equal(out.isnan().any(-1).any(-1).cpu(), sees)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_pages_past_32_bits(ops, dev, bits):
+    """Pages a gigabyte apart (offsets past 2^32 bytes): every operator bit for bit as over a dense cache."""
+    heads, group, d, page = 2, 4, 64, 32
+    new, before = [1, 40, 3], [60, 30, 0]
+    lens = [a + b for a, b in zip(new, before)]
+    c = P.Cache(lens, heads, d, d, page, BF, bits)
+    held = c.to(dev)
+    pages = held["k_cache"].size(0)
+    assert pages >= 6
+    far = dict(held)
+    step = 2**29 if bits == 16 else 2**30 - 16
+    span = heads * page * held["k_cache"].size(3)
+    store = torch.empty(step * (pages - 1) + 2 * span, dtype=held["k_cache"].dtype, device=dev)
+    for n, first in (("k_cache", 0), ("v_cache", span)):
+        x = held[n]
+        far[n] = torch.as_strided(store, x.shape, (step, page * x.size(3), x.size(3), 1), first)
+        far[n].copy_(x)
+    cu = torch.tensor(P.cu_of(new), dtype=torch.int32, device=dev)
+    t = sum(new)
+    k, v, q = (_randn(t, n, d, seed=s, dtype=BF).to(dev) for n, s in ((heads, 1), (heads, 2), (heads * group, 3)))
+    freq = _freq(d // 2).to(dev)
+    qr = [ops.paged_append(k, v, **h, cu_seq=cu, q=q, inv_freq=freq) for h in (held, far)]
+    assert torch.equal(qr[0], qr[1])
+    for n in held:
+        assert torch.equal(held[n].contiguous().view(torch.uint8), far[n].contiguous().view(torch.uint8)), n
+    for args in ({"cu_seq_q": cu, "max_q": max(new)}, {"cu_seq_q": cu, "max_q": 1}, {}):
+        qq = qr[0] if args else qr[0][: len(new)]
+        one, two = (ops.sdpa_paged(qq, **h, **args, max_k=max(lens)) for h in (held, far))
+        if args.get("max_q") == 1:
+            one, two = one[cu[:-1].long()], two[cu[:-1].long()]
+        assert torch.equal(one, two)
+    scales = {n: held[n] for n in held if n.endswith("scale")}
+    one, two = (ops.paged_read(h["k_cache"], h["v_cache"], h["block_table"], h["key_lengths"], max(lens), **scales)
+                for h in (held, far))
+    assert torch.equal(one[0], two[0]) and torch.equal(one[1], two[1])
+
+
 @pytest.mark.parametrize("bits", [16, 4])
 def test_default_bounds_and_a_wide_table(ops, dev, bits):
     """max_k from the table's width (far more than any length), strided q and table."""
