@@ -77,29 +77,27 @@ struct AttnParams : fwd::AttnParams {
 };
 
 // Zeros (and log-sum-exps of minus infinity) for the rows behind the last sequence, in a split
-// call through the merge, by the call's tail_blocks last workgroups.
+// call through the merge, by tail_blocks workgroups of the call.
 template <typename T>
 __device__ __forceinline__ void zero_tail(const AttnParams& p, int block) {
-    const int t0 = min(max(uniform_i32(p.c.cu + p.c.batch), 0), p.c.tokens);
-    const int vec = p.dv / 4;
-    const int64_t first = static_cast<int64_t>(block) * blockDim.x + threadIdx.x;
-    const int64_t stride = static_cast<int64_t>(p.tail_blocks) * blockDim.x;
-    const int64_t n = static_cast<int64_t>(p.c.tokens - t0) * p.hq;
-    if (p.splits > 1) {
-        for (int64_t i = first; i < n * p.splits; i += stride) {
-            const int64_t s = i / n;
-            p.part_lse[(s * p.rows_total + t0) * p.hq + (i - s * n)] = -INFINITY;
-        }
-        return;
-    }
     typedef T t4 __attribute__((ext_vector_type(4)));
-    for (int64_t i = first; i < n * vec; i += stride) {
-        const int64_t r = i / vec, t = t0 + r / p.hq, h = r % p.hq;
-        *reinterpret_cast<t4*>(static_cast<T*>(p.out) + t * p.os[2] + h * p.os[1] + 4 * (i - r * vec)) = t4{};
+    const int vec = p.dv / 4;
+    for (int t = min(max(uniform_i32(p.c.cu + p.c.batch), 0), p.c.tokens) + block; t < p.c.tokens; t += p.tail_blocks) {
+        if (p.splits > 1) {
+            for (int i = threadIdx.x; i < p.hq * p.splits; i += blockDim.x) {
+                const int s = i / p.hq;
+                p.part_lse[(s * p.rows_total + t) * p.hq + (i - s * p.hq)] = -INFINITY;
+            }
+            continue;
+        }
+        T* const row = static_cast<T*>(p.out) + t * p.os[2];
+        for (int i = threadIdx.x; i < p.hq * vec; i += blockDim.x) {
+            const int h = i / vec;
+            *reinterpret_cast<t4*>(row + h * p.os[1] + 4 * (i - h * vec)) = t4{};
+        }
+        if (p.lse)
+            for (int h = threadIdx.x; h < p.hq; h += blockDim.x) p.lse[t * p.ls[2] + h * p.ls[1]] = -INFINITY;
     }
-    if (p.lse)
-        for (int64_t r = first; r < n; r += stride)
-            p.lse[(t0 + r / p.hq) * p.ls[2] + (r % p.hq) * p.ls[1]] = -INFINITY;
 }
 
 // Enqueues a call's kernel (the merge is paged_attention.hip's).  rows: 16 or 32 virtual rows a

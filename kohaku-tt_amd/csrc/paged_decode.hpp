@@ -128,12 +128,13 @@ __global__ __launch_bounds__(THREADS, decode_occupancy(DP, NQ, FOUR)) void paged
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g4 = lane >> 4, l16 = lane & 15;
     const int units = p.batch * p.hkv;
-    if (static_cast<int>(blockIdx.x) >= units * p.splits) {
-        zero_tail<T>(p, blockIdx.x - units * p.splits);
+    const int lin = static_cast<int>(blockIdx.x) - p.tail_blocks;
+    if (lin < 0) {
+        zero_tail<T>(p, blockIdx.x);
         return;
     }
-    const int bh = fwd::fdiv(static_cast<int>(blockIdx.x), p.fd_splits);
-    const int split = blockIdx.x - bh * p.splits;
+    const int bh = fwd::fdiv(lin, p.fd_splits);
+    const int split = lin - bh * p.splits;
     const int seq = fwd::fdiv(bh, p.fd_hkv), kvh = bh - seq * p.hkv;
     const int G = p.group;
     // Tiles are dealt to a unit's wavefronts in turn: tile slot, slot + nslots, ...  A wavefront's
@@ -506,7 +507,6 @@ __global__ __launch_bounds__(THREADS, decode_occupancy(DP, NQ, FOUR)) void paged
             }
         }
         const float inv = total == 0.f ? 0.f : 1.f / total;
-        const float log = total == 0.f ? -INFINITY : top + log2f(total);
         const int64_t tok = sp.q0 + pos[n];
         if (p.splits == 1) {
             T* dst = static_cast<T*>(p.out) + head[n] * p.os[1] + tok * p.os[2] + c0;
@@ -519,7 +519,7 @@ __global__ __launch_bounds__(THREADS, decode_occupancy(DP, NQ, FOUR)) void paged
                 if (c0 + i < p.dv) *reinterpret_cast<tper*>(dst + i) = y;
             }
             if (p.lse && wave == 0 && g4 == 0)
-                p.lse[head[n] * p.ls[1] + tok * p.ls[2]] = log * kLn2f;
+                p.lse[head[n] * p.ls[1] + tok * p.ls[2]] = total == 0.f ? -INFINITY : (top + log2f(total)) * kLn2f;
         } else {
             const int64_t at = (static_cast<int64_t>(split) * p.rows_total + tok) * p.hq + head[n];
 #pragma unroll
@@ -529,7 +529,7 @@ __global__ __launch_bounds__(THREADS, decode_occupancy(DP, NQ, FOUR)) void paged
                 for (int e = 0; e < VE; ++e) y[e] = acc[i + e] * inv;
                 if (c0 + i < p.dv) *reinterpret_cast<fper*>(p.part_o + at * DP + c0 + i) = y;
             }
-            if (wave == 0 && g4 == 0) p.part_lse[at] = log;
+            if (wave == 0 && g4 == 0) p.part_lse[at] = total == 0.f ? -INFINITY : top + log2f(total);
         }
     }
 }
