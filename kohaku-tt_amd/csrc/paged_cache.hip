@@ -11,6 +11,7 @@
 //
 // Read: four 16-byte stores a thread, their rows found through the table.
 #include <algorithm>
+#include <cmath>
 
 #include "paged.hpp"
 
@@ -105,6 +106,7 @@ struct AppendParams {
     int hq, rd, inter;
     const float* freq;
     double scale;
+    float slack;  // 2^-21 |scale|: what rotated values are off in 32 bits, of their pair's sizes
     int nk, nv;    // chunks of a query or key row, of a value row
     // Workgroups of queries and keys come first, those of values behind them: items (vectors, or
     // pairs of them) of a token and tokens of a workgroup for each.
@@ -112,17 +114,20 @@ struct AppendParams {
     fwd::FastDiv fd_qk, fd_v, fd_nk, fd_nv, fd_half;
 };
 
-// A token's page (-1: none), row there and position (-1: none).
+// A token's row in head 0 of the cache and its scales there, in bytes (-1: none), and its position
+// (-1: none).
 struct Held {
-    int page, row, pos, pad;
+    int64_t at, scale;
+    int pos, pad;
 };
 
 // The places of a workgroup's tokens and, for rotated calls, their angles' cosines and sines (F:
-// float or double), into LDS.  Tokens of one sequence (nearly every workgroup's) find it by scalar
+// float, or double, then in both), into LDS.  Tokens of one sequence (nearly every workgroup's) find it by scalar
 // loads, which do not queue behind the vectors in flight, and wait for one vector load, the
 // table's; a workgroup across sequences searches per token.
 template <typename F>
-__device__ __forceinline__ void place_tokens(const AppendParams& p, int t0, int nt, Held* held, F* cosine, F* sine) {
+__device__ __forceinline__ void place_tokens(const AppendParams& p, const int64_t (&st)[3], const int64_t (&ss)[3], int t0, int nt, Held* held, float* cosine,
+                                             float* sine, F* cosine_f = nullptr, F* sine_f = nullptr) {
     const Cache& c = p.c;
     const int half = cosine ? p.rd / 2 : 0;
     int seq = t0, first = 0, lq = 1;
@@ -150,8 +155,13 @@ __device__ __forceinline__ void place_tokens(const AppendParams& p, int t0, int 
             at = place_of(c, t0 + threadIdx.x);
         else if (pos0 + threadIdx.x >= 0 && pos0 + threadIdx.x < c.capacity)
             at.pos = static_cast<int>(pos0 + threadIdx.x);
-        Held h{-1, 0, at.pos, 0};
-        if (at.pos >= 0) h.page = page_of(c, at.seq, at.pos, h.row);
+        Held h{-1, -1, at.pos, 0};
+        int row;
+        const int64_t page = at.pos >= 0 ? page_of(c, at.seq, at.pos, row) : -1;
+        if (page >= 0) {
+            h.at = page * st[0] + row * st[2];
+            h.scale = page * ss[0] + row * ss[2];
+        }
         held[threadIdx.x] = h;
     }
     if (!one) __syncthreads();  // (uniform)
@@ -160,8 +170,14 @@ __device__ __forceinline__ void place_tokens(const AppendParams& p, int t0, int 
         const double pos = one ? static_cast<double>(pos0 + tl) : static_cast<double>(held[tl].pos);
         F cs, sn;
         turn(pos, p.freq[i - tl * half], cs, sn);
-        cosine[i] = cs * static_cast<F>(p.scale);
-        sine[i] = sn * static_cast<F>(p.scale);
+        cs *= static_cast<F>(p.scale);
+        sn *= static_cast<F>(p.scale);
+        cosine[i] = static_cast<float>(cs);
+        sine[i] = static_cast<float>(sn);
+        if constexpr (std::is_same<F, double>::value) {
+            cosine_f[i] = cs;
+            sine_f[i] = sn;
+        }
     }
     __syncthreads();
 }
@@ -188,10 +204,10 @@ __device__ __forceinline__ const T* qk_row(const AppendParams& p, int64_t t, int
                     : static_cast<const T*>(p.k) + t * p.ks[0] + (h - p.hq) * p.ks[1];
 }
 __device__ __forceinline__ char* k_place(const AppendParams& p, const Held& at, int h) {
-    return p.c.k + at.page * p.c.ks[0] + h * p.c.ks[1] + at.row * p.c.ks[2];
+    return p.c.k + at.at + h * p.c.ks[1];
 }
 __device__ __forceinline__ char* v_place(const AppendParams& p, const Held& at, int h) {
-    return p.c.v + at.page * p.c.vs[0] + h * p.c.vs[1] + at.row * p.c.vs[2];
+    return p.c.v + at.at + h * p.c.vs[1];
 }
 
 template <typename T>
@@ -225,14 +241,14 @@ __device__ __forceinline__ void append_values(const AppendParams& p, int block, 
             x[j] = *reinterpret_cast<const V8<T>*>(static_cast<const T*>(p.v) + static_cast<int64_t>(t0 + m.tl) * p.vs[0] +
                                                    m.h * p.vs[1] + 8 * m.c);
         }
-        if (base == 0) place_tokens<float>(p, t0, nt, held, nullptr, nullptr);
+        if (base == 0) place_tokens<float>(p, p.c.vs, p.c.vss, t0, nt, held, nullptr, nullptr);
 #pragma unroll
         for (int j = 0; j < ITEMS; ++j) {
             const int i = base + j * THREADS + threadIdx.x;
             if (i >= items) break;
             const Item m = v_item(p, i);
             const Held at = held[m.tl];
-            if (at.page >= 0) out(at, m.h, m.c, x[j]);
+            if (at.at >= 0) out(at, m.h, m.c, x[j]);
         }
     }
 }
@@ -277,7 +293,7 @@ __global__ __launch_bounds__(THREADS) void append_kernel(const AppendParams p) {
         }
     };
     fetch(0);
-    place_tokens(p, t0, nt, held, cosine, sine);
+    place_tokens<float>(p, p.c.ks, p.c.kss, t0, nt, held, cosine, sine);
     for (int base = 0;;) {
 #pragma unroll
         for (int j = 0; j < ITEMS; ++j) {
@@ -291,7 +307,7 @@ __global__ __launch_bounds__(THREADS) void append_kernel(const AppendParams p) {
                 // A query of no sequence (or past the cache) is zero.
                 if (at.pos < 0) a[j] = z[j] = Vec{};
             } else {
-                if (at.page < 0) continue;
+                if (at.at < 0) continue;
                 dst = reinterpret_cast<T*>(k_place(p, at, m.h - p.hq));
             }
             dst += first_dim(m.c);
@@ -330,14 +346,14 @@ __global__ __launch_bounds__(THREADS) void append_kernel(const AppendParams p) {
 
 // ---------------------------------------------------------------- 4 bits
 
-// The largest of a value over the four lanes of a group.
+// The largest of a value (not negative) over the four lanes of a group: a quad's exchanges.
 __device__ __forceinline__ int max_of_four(int v) {
-    v = max(v, __shfl_xor(v, 1, kWave));
-    return max(v, __shfl_xor(v, 2, kWave));
+    v = max(v, __builtin_amdgcn_mov_dpp(v, 0xb1, 0xf, 0xf, true));  // lanes 1, 0, 3, 2
+    return max(v, __builtin_amdgcn_mov_dpp(v, 0x4e, 0xf, 0xf, true));  // lanes 2, 3, 0, 1
 }
 
-// The group's scale byte and 2^-e from the largest exponent field (biased by `bias`, `top_field`
-// for infinities and NaN) of its values.
+// The group's scale byte and exponent e from the largest exponent field (biased by `bias`,
+// `top_field` for infinities and NaN) of its values.
 struct Scale {
     int byte, e;
 };
@@ -347,76 +363,105 @@ __device__ __forceinline__ Scale group_scale(int field, int bias, int top_field)
     return Scale{field == top_field ? 255 : e + 127, e};
 }
 
-// Eight values in units of the scale as codes: nearest, ties to even, saturating.
-__device__ __forceinline__ uint32_t codes_of(const float (&f)[8]) {
-    uint32_t codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, f[0], f[1], 1.f, 0);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, f[2], f[3], 1.f, 1);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, f[4], f[5], 1.f, 2);
-    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, f[6], f[7], 1.f, 3);
+// Eight values over a power of two as codes: nearest, ties to even, saturating.
+__device__ __forceinline__ uint32_t codes_of(const float (&f)[8], float unit) {
+    uint32_t codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, f[0], f[1], unit, 0);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, f[2], f[3], unit, 1);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, f[4], f[5], unit, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, f[6], f[7], unit, 3);
+}
+// (Through a dword of its own: a vector's element in a bit cast stands for the first one.)
+__device__ __forceinline__ uint32_t codes_of(const bf16x8& x, float unit) {
+    typedef __bf16 pair __attribute__((ext_vector_type(2)));
+    const u32x4 w = __builtin_bit_cast(u32x4, x);
+    const uint32_t a = w[0], b = w[1], c = w[2], d = w[3];
+    uint32_t codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(0u, __builtin_bit_cast(pair, a), unit, 0);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(codes, __builtin_bit_cast(pair, b), unit, 1);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(codes, __builtin_bit_cast(pair, c), unit, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(codes, __builtin_bit_cast(pair, d), unit, 3);
+}
+__device__ __forceinline__ uint32_t codes_of(const f16x8& x, float unit) {
+    typedef _Float16 pair __attribute__((ext_vector_type(2)));
+    const u32x4 w = __builtin_bit_cast(u32x4, x);
+    const uint32_t a = w[0], b = w[1], c = w[2], d = w[3];
+    uint32_t codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(0u, __builtin_bit_cast(pair, a), unit, 0);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(codes, __builtin_bit_cast(pair, b), unit, 1);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(codes, __builtin_bit_cast(pair, c), unit, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(codes, __builtin_bit_cast(pair, d), unit, 3);
 }
 
-// Values of 16 bits: exact in 32 bits, and so is their product with a power of two (values that
-// vanish below 2^-149 are zeros in any code).
+// Values of 16 bits, converted as they are: their largest by its bits, two at a time.
 template <typename T>
 __device__ __forceinline__ uint32_t quantise(const V8<T>& x, int& byte) {
-    float f[8];
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        f[i] = to_f32(x[i]);
-        top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
-    }
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    const u32x4 w = __builtin_bit_cast(u32x4, x) & 0x7fff7fffu;
+    const uint32_t a = w[0], b = w[1], c = w[2], d = w[3];
+    const u16x2 two = __builtin_elementwise_max(
+        __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)),
+        __builtin_elementwise_max(__builtin_bit_cast(u16x2, c), __builtin_bit_cast(u16x2, d)));
+    const int top = max_of_four(max(static_cast<int>(two[0]), static_cast<int>(two[1])));
+    const float largest = to_f32(__builtin_bit_cast(T, static_cast<uint16_t>(top)));
     // (A subnormal bf16's exponent is below the smallest scale's, as a field of zero says; only
     // zero itself keeps the byte 0.)
-    const int nonzero = max_of_four(top != 0);
-    Scale s = group_scale(static_cast<int>(top >> 23), 127, 255);
-    if (nonzero && s.byte == 0) s = Scale{1, -126};
-    byte = s.byte;
-    // 2^-e in two factors: e reaches 127.
-    const float a = __uint_as_float(static_cast<uint32_t>(127 - s.e / 2) << 23);
-    const float b = __uint_as_float(static_cast<uint32_t>(127 - (s.e - s.e / 2)) << 23);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = f[i] * a * b;
-    return codes_of(f);
+    const int field = static_cast<int>(__float_as_uint(largest) >> 23);
+    byte = field == 255 ? 255 : max(field - 2, top == 0 ? 0 : 1);
+    return codes_of(x, scale_of(max(byte, 1)));
 }
 
-// Rotated values in 64 bits: the codes are those nearest to y 2^-e in exact arithmetic.  The
-// product is exact in 64 bits and rounds to 32 toward zero with the last bit set where that drops
-// anything, which no border between two codes has (nearest rounding could land on one).
-__device__ __forceinline__ uint32_t quantise(const double (&y)[8], int& byte) {
-    int top = 0;
+// A value of 64 bits in 32, toward zero with the last bit set where that drops anything: no border
+// between two codes has that bit (nearest rounding could land on one), so codes stay those of the
+// value as it was.
+__device__ __forceinline__ float to_odd(double x) {
+    const float f = static_cast<float>(x);
+    const double back = static_cast<double>(f);
+    const uint32_t bits = __float_as_uint(f);
+    return back == x ? f : __uint_as_float((fabs(back) > fabs(x) ? bits - 1 : bits) | 1u);
+}
+
+// Rotated values in 32 bits, each at most `slack` off the exact one: their codes, should they be
+// those of every value that near (`sure`, the same for the lanes of a group), so that the nearest
+// codes in exact arithmetic cost 64 bits only next to a border (one group in some thousands).
+__device__ __forceinline__ uint32_t quantise(const float (&y)[8], float slack, int& byte, bool& sure) {
+    float top = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, static_cast<int>(__double2hiint(y[i]) & 0x7fffffff));
-    const Scale s = group_scale(top >> 20, 1023, 0x7ff);
-    byte = s.byte;
-    const double inv = __hiloint2double((1023 - s.e) << 20, 0);
-    float f[8];
+    for (int i = 0; i < 8; ++i) top = __uint_as_float(max(__float_as_uint(top), __float_as_uint(y[i]) & 0x7fffffffu));
+    // The group's largest lies between these two.
+    const int most = max_of_four(__float_as_int(top + slack)), least = max_of_four(__float_as_int(fmaxf(top - slack, 0.f)));
+    const int field = most >> 23;
+    // (Within them nothing that counts is subnormal, scale and slack included.)
+    const bool plain = field == least >> 23 && ((field >= 60 && field <= 150) || most == 0);
+    byte = most == 0 ? 0 : field - 2;
+    const float unit = scale_of(max(byte, 1));
+    float lo[8], hi[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const double x = y[i] * inv;
-        f[i] = static_cast<float>(x);
-        const double back = static_cast<double>(f[i]);
-        if (back != x) {
-            const uint32_t bits = __float_as_uint(f[i]);
-            f[i] = __uint_as_float((fabs(back) > fabs(x) ? bits - 1 : bits) | 1u);
-        }
+        lo[i] = y[i] - slack;
+        hi[i] = y[i] + slack;
     }
-    return codes_of(f);
+    const uint32_t codes = codes_of(lo, unit);
+    // (A slack of zero leaves the sign of zeros alone in lo.)
+    sure = max_of_four(plain && (codes == codes_of(hi, unit) || slack == 0.f) ? 0 : 1) == 0;
+    return codes;
 }
 
 // Chunks of eight dims; head dims are whole groups, so a group's four chunks are four
 // neighbouring lanes with items of one token and head.
+//
+// Bound by issue (the vector unit was busy 78% of the time) until keys were rotated and converted in
+// 32 bits, values converted as they are, and rows' places formed once a token: 4 x up to 2048 tokens
+// of 8 heads x 128 18.3 to 14.3 us in a graph, 4 x 4096 36.4 to 26.0 (3.3 TB/s).  The 64-bit groups
+// read their vectors at once: value after value they took the call back to 20 us.
 template <typename T, bool INTER>
 __global__ __launch_bounds__(THREADS) void append4_kernel(const AppendParams p) {
-    __shared__ __align__(16) double cosine[PAIRS], sine[PAIRS];
+    __shared__ __align__(32) float cosine[PAIRS], sine[PAIRS];
+    __shared__ __align__(16) double cosine64[PAIRS], sine64[PAIRS];
     __shared__ Held held[TOKENS];
     typedef V8<T> v8;
     if (static_cast<int>(blockIdx.x) >= p.blocks_qk) {
         append_values<T>(p, blockIdx.x - p.blocks_qk, held, [&](const Held& at, int h, int c, const v8& x) {
             int byte;
             *reinterpret_cast<uint32_t*>(v_place(p, at, h) + 4 * c) = quantise<T>(x, byte);
-            if ((c & 3) == 0)
-                p.c.vsc[at.page * p.c.vss[0] + h * p.c.vss[1] + at.row * p.c.vss[2] + (c >> 2)] = static_cast<uint8_t>(byte);
+            if ((c & 3) == 0) p.c.vsc[at.scale + h * p.c.vss[1] + (c >> 2)] = static_cast<uint8_t>(byte);
         });
         return;
     }
@@ -424,8 +469,9 @@ __global__ __launch_bounds__(THREADS) void append4_kernel(const AppendParams p) 
     const int nt = min(p.tpb_qk, p.c.tokens - t0);
     const int items = nt * p.per_qk;
     const int half = p.rd / 2;
-    // Half layout: whole partner vectors where a half is a number of chunks.
-    const bool whole = half % 8 == 0;
+    // Rotated dims that are whole chunks (their halves, unless pairs are neighbours): a chunk's
+    // partners are one then too, and all of it is rotated, or none.
+    const bool whole = INTER ? p.rd % 8 == 0 : half % 8 == 0;
     v8 x[ITEMS], z[ITEMS];
     auto fetch = [&](int base) {
 #pragma unroll
@@ -436,53 +482,105 @@ __global__ __launch_bounds__(THREADS) void append4_kernel(const AppendParams p) 
             const T* src = qk_row<T>(p, t0 + m.tl, m.h);
             const int d0 = 8 * m.c;
             x[j] = *reinterpret_cast<const v8*>(src + d0);
-            if (INTER || d0 >= p.rd) continue;
-            if (whole) {
-                z[j] = *reinterpret_cast<const v8*>(src + (d0 < half ? d0 + half : d0 - half));
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int d = d0 + e;
-                    z[j][e] = d < p.rd ? src[d < half ? d + half : d - half] : x[j][e];
-                }
-            }
+            if (!INTER && whole && d0 < p.rd) z[j] = *reinterpret_cast<const v8*>(src + (d0 < half ? d0 + half : d0 - half));
         }
     };
+    const auto keep = [&](const Item& m, const Held& at, uint32_t codes, int byte) {
+        const int h = m.h - p.hq;
+        *reinterpret_cast<uint32_t*>(k_place(p, at, h) + 4 * m.c) = codes;
+        if ((m.c & 3) == 0) p.c.ksc[at.scale + h * p.c.kss[1] + (m.c >> 2)] = static_cast<uint8_t>(byte);
+    };
+    const auto q_place = [&](const Item& m) {
+        return static_cast<T*>(p.qo) + static_cast<int64_t>(t0 + m.tl) * p.qos[0] + m.h * p.qos[1] + 8 * m.c;
+    };
     fetch(0);
-    place_tokens(p, t0, nt, held, cosine, sine);
+    place_tokens<double>(p, p.c.ks, p.c.kss, t0, nt, held, cosine, sine, cosine64, sine64);
     for (int base = 0;;) {
+        uint32_t again = 0;
 #pragma unroll
         for (int j = 0; j < ITEMS; ++j) {
             const int i = base + j * THREADS + threadIdx.x;
             if (i >= items) break;
             const Item m = qk_item(p, i);
             const Held at = held[m.tl];
-            if (m.h >= p.hq && at.page < 0) continue;  // (all four lanes of a group)
+            if (m.h >= p.hq && at.at < 0) continue;  // (all four lanes of a group)
+            if (!whole) {
+                again |= 1u << j;
+                continue;
+            }
             const int d0 = 8 * m.c;
-            double y[8];
+            float y[8], size = 0.f;
+            if (d0 < p.rd) {
+                constexpr int N = INTER ? 4 : 8;  // angles
+                const bool front = d0 < half;
+                const int k = m.tl * half + (INTER ? d0 / 2 : (front ? d0 : d0 - half));
+                float c[N], s[N];
+                __builtin_memcpy(c, __builtin_assume_aligned(cosine + k, 4 * N), 4 * N);
+                __builtin_memcpy(s, __builtin_assume_aligned(sine + k, 4 * N), 4 * N);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int d = d0 + e;
-                y[e] = static_cast<double>(to_f32(x[j][e]));
-                if (d >= p.rd) continue;
-                // Its value times the cosine plus or minus its partner's times the sine.
-                const bool first = INTER ? (e & 1) == 0 : d < half;
-                const int k = m.tl * half + (INTER ? d >> 1 : (first ? d : d - half));
-                const double other = static_cast<double>(to_f32(INTER ? x[j][e ^ 1] : z[j][e]));
-                y[e] = y[e] * cosine[k] + other * (first ? -sine[k] : sine[k]);
+                for (int e = 0; e < 8; ++e) {
+                    const float own = to_f32(x[j][e]), other = to_f32(INTER ? x[j][e ^ 1] : z[j][e]);
+                    const float t = other * s[INTER ? e >> 1 : e];
+                    const bool minus = INTER ? (e & 1) == 0 : front;
+                    y[e] = __builtin_fmaf(own, c[INTER ? e >> 1 : e], minus ? -t : t);
+                    size = fmaxf(size, fabsf(own) + fabsf(other));
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = to_f32(x[j][e]);
             }
             if (m.h < p.hq) {
                 v8 w;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) w[e] = from_f32<T>(at.pos < 0 ? 0.f : static_cast<float>(y[e]));
-                *reinterpret_cast<v8*>(static_cast<T*>(p.qo) + static_cast<int64_t>(t0 + m.tl) * p.qos[0] + m.h * p.qos[1] + d0) = w;
+                for (int e = 0; e < 8; ++e) w[e] = from_f32<T>(at.pos < 0 ? 0.f : y[e]);
+                *reinterpret_cast<v8*>(q_place(m)) = w;
                 continue;
             }
+            // Off by the cosine's and sine's rounding, the product's and the sum's, each 2^-24 of
+            // (|x| + |other|) scale at most, doubled for what the test itself rounds.
             int byte;
-            const int h = m.h - p.hq;
-            *reinterpret_cast<uint32_t*>(k_place(p, at, h) + 4 * m.c) = quantise(y, byte);
-            if ((m.c & 3) == 0)
-                p.c.ksc[at.page * p.c.kss[0] + h * p.c.kss[1] + at.row * p.c.kss[2] + (m.c >> 2)] = static_cast<uint8_t>(byte);
+            bool sure;
+            const uint32_t codes = quantise(y, size == 0.f ? 0.f : fmaxf(size * p.slack, 0x1p-100f), byte, sure);
+            if (sure)
+                keep(m, at, codes, byte);
+            else
+                again |= 1u << j;
+        }
+        // Groups next to a border, and rotated dims that are no whole chunks: in 64 bits, value by
+        // value from memory.
+#pragma unroll 1
+        for (int j = 0; again != 0; ++j, again >>= 1) {
+            if ((again & 1u) == 0) continue;
+            const Item m = qk_item(p, base + j * THREADS + threadIdx.x);
+            const Held at = held[m.tl];
+            const T* const src = qk_row<T>(p, t0 + m.tl, m.h);
+            const auto value = [&](int d) {
+                const double own = static_cast<double>(to_f32(src[d]));
+                if (d >= p.rd) return own;
+                const bool first = INTER ? (d & 1) == 0 : d < half;
+                const double other = static_cast<double>(to_f32(src[INTER ? d ^ 1 : (first ? d + half : d - half)]));
+                const int k = m.tl * half + (INTER ? d >> 1 : (first ? d : d - half));
+                return own * cosine64[k] + other * (first ? -sine64[k] : sine64[k]);
+            };
+            double y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = value(8 * m.c + e);
+            if (m.h < p.hq) {
+                v8 w;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] = from_f32<T>(at.pos < 0 ? 0.f : static_cast<float>(y[e]));
+                *reinterpret_cast<v8*>(q_place(m)) = w;
+                continue;
+            }
+            int top = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = max(top, static_cast<int>(__double2hiint(y[e]) & 0x7fffffff));
+            const Scale scale = group_scale(top >> 20, 1023, 0x7ff);
+            const double inv = __hiloint2double((1023 - scale.e) << 20, 0);
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = to_odd(y[e] * inv);
+            keep(m, at, codes_of(f, 1.f), scale.byte);
         }
         base += ITEMS * THREADS;
         if (base >= items) break;
@@ -531,6 +629,7 @@ hipError_t launch_append(const kmi_paged_append_args* a, hipStream_t stream) {
     p.inter = a->interleaved ? 1 : 0;
     p.freq = a->inv_freq;
     p.scale = a->rotary_scale;
+    p.slack = static_cast<float>(std::fabs(a->rotary_scale) * 0x1p-21);
     const int64_t tokens = a->cache.tokens;
     const bool four = a->cache.bits == 4;
     const int vw = four ? 8 : (p.rd % 16 == 0 ? 8 : 1);
