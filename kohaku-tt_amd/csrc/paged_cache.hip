@@ -662,58 +662,75 @@ hipError_t launch_append(const kmi_paged_append_args* a, hipStream_t stream) {
 
 // ---------------------------------------------------------------- read
 
-struct ReadParams {
-    Cache c;
-    void* k;
-    void* v;
-    int max_k, nk, nv;  // chunks of eight dims
-    int blocks;         // workgroups per (sequence, K/V head)
+// Keys or values: where they lie, and the dense copy.
+struct Side {
+    const char* rows;
+    const uint8_t* scales;
+    int64_t stride[3], scale_stride[3];
+    char* out;
+    int chunks;  // of eight dims, of a row
+    int blocks;  // workgroups per (sequence, K/V head)
     fwd::FastDiv fd_chunks;
 };
 
+struct ReadParams {
+    Cache c;
+    Side side[2];
+    int max_k;
+};
+
+// A workgroup copies chunks of one unit's keys or values.
 template <typename T, bool FOUR>
 __global__ __launch_bounds__(THREADS) void read_kernel(const ReadParams p) {
-    const int unit = blockIdx.x / p.blocks;
+    const int per = p.side[0].blocks + p.side[1].blocks;
+    const int unit = blockIdx.x / per;
     const int b = unit / p.c.hkv, h = unit - b * p.c.hkv;
-    const int first = (blockIdx.x - unit * p.blocks) * (THREADS * ITEMS) + threadIdx.x;
+    int block = blockIdx.x - unit * per;
+    const bool values = block >= p.side[0].blocks;
+    const Side& side = p.side[values ? 1 : 0];
+    if (values) block -= p.side[0].blocks;
+    const int first = block * (THREADS * ITEMS) + threadIdx.x;
     const int lk = min(max(uniform_i32(p.c.klen + b), 0), p.c.capacity);
     u32x4 x[ITEMS];
     uint32_t byte[ITEMS];
     int pos[ITEMS], c[ITEMS], entry[ITEMS], row[ITEMS];
-    bool key[ITEMS];
 #pragma unroll
     for (int j = 0; j < ITEMS; ++j) {
-        pos[j] = fwd::fdiv(first + j * THREADS, p.fd_chunks);
-        c[j] = first + j * THREADS - pos[j] * (p.nk + p.nv);
-        key[j] = c[j] < p.nk;
-        if (!key[j]) c[j] -= p.nk;
+        pos[j] = fwd::fdiv(first + j * THREADS, side.fd_chunks);
+        c[j] = first + j * THREADS - pos[j] * side.chunks;
         x[j] = u32x4{0u, 0u, 0u, 0u};
         byte[j] = 0;
     }
     if (lk > 0) {
         // Every table entry, then every row (keys past the last repeat its, unused), so that a
         // thread's items wait for memory together.
+        const int32_t* const table = p.c.table + b * p.c.table_stride;
 #pragma unroll
         for (int j = 0; j < ITEMS; ++j) {
             const int at = min(pos[j], lk - 1), n = fwd::fdiv(at, p.c.fd_page);
             row[j] = at - n * p.c.page;
-            entry[j] = p.c.table[b * p.c.table_stride + n];
+            entry[j] = table[n];
         }
+        const char* const rows = side.rows + h * side.stride[1];
+        const uint8_t* const scales = side.scales + h * side.scale_stride[1];
 #pragma unroll
         for (int j = 0; j < ITEMS; ++j) {
-            const int page = clamp_page(entry[j], p.c.pages);
-            const char* src = key[j] ? p.c.k + page * p.c.ks[0] + h * p.c.ks[1] + row[j] * p.c.ks[2]
-                                     : p.c.v + page * p.c.vs[0] + h * p.c.vs[1] + row[j] * p.c.vs[2];
+            // (Page strides are below 2^32 bytes, row strides below 2^26.)
+            const uint32_t page = static_cast<uint32_t>(clamp_page(entry[j], p.c.pages)), r = static_cast<uint32_t>(row[j]);
+            const auto at = [&](const int64_t(&st)[3], uint32_t inner) {
+                return static_cast<uint64_t>(page) * static_cast<uint32_t>(st[0]) +
+                       static_cast<uint64_t>(r) * static_cast<uint32_t>(st[2]) + inner;
+            };
+            const uint32_t chunk = static_cast<uint32_t>(c[j]);
             if constexpr (FOUR) {
-                const uint8_t* sc = key[j] ? p.c.ksc + page * p.c.kss[0] + h * p.c.kss[1] + row[j] * p.c.kss[2]
-                                           : p.c.vsc + page * p.c.vss[0] + h * p.c.vss[1] + row[j] * p.c.vss[2];
-                byte[j] = sc[c[j] >> 2];
-                x[j][0] = *reinterpret_cast<const uint32_t*>(src + 4 * c[j]);
+                byte[j] = scales[at(side.scale_stride, chunk >> 2)];
+                x[j][0] = *reinterpret_cast<const uint32_t*>(rows + at(side.stride, 4 * chunk));
             } else {
-                x[j] = *reinterpret_cast<const u32x4*>(src + 16 * c[j]);
+                x[j] = *reinterpret_cast<const u32x4*>(rows + at(side.stride, 16 * chunk));
             }
         }
     }
+    char* const out = side.out + static_cast<int64_t>(unit) * p.max_k * (side.chunks * 16);
 #pragma unroll
     for (int j = 0; j < ITEMS; ++j) {
         if (pos[j] >= p.max_k) continue;
@@ -724,26 +741,32 @@ __global__ __launch_bounds__(THREADS) void read_kernel(const ReadParams p) {
             for (int e = 0; e < 4; ++e) x[j][e] = fp4_pair<T>(codes, s, e);
         }
         if (pos[j] >= lk) x[j] = u32x4{0u, 0u, 0u, 0u};
-        char* dst = static_cast<char*>(key[j] ? p.k : p.v);
-        *reinterpret_cast<u32x4*>(dst + ((static_cast<int64_t>(unit) * p.max_k + pos[j]) * (key[j] ? p.nk : p.nv) + c[j]) * 16) = x[j];
+        *reinterpret_cast<u32x4*>(out + static_cast<uint64_t>(static_cast<uint32_t>(first + j * THREADS)) * 16) = x[j];
     }
 }
 
 }  // namespace
 
-hipError_t launch_read(const kmi_paged_cache& cache, void* k, void* v, int64_t max_k, hipStream_t stream) {
+hipError_t launch_read(const kmi_paged_cache& c, void* k, void* v, int64_t max_k, hipStream_t stream) {
     ReadParams p{};
-    p.c = device_cache(cache);
-    p.k = k;
-    p.v = v;
+    p.c = device_cache(c);
     p.max_k = static_cast<int>(max_k);
-    p.nk = p.c.d / 8;
-    p.nv = p.c.dv / 8;
-    p.fd_chunks = fwd::fast_div(static_cast<uint32_t>(p.nk + p.nv));
-    p.blocks = static_cast<int>(ceil_div(max_k * (p.nk + p.nv), THREADS * ITEMS));
-    const dim3 grid(static_cast<unsigned>(p.blocks * cache.batch * cache.heads_kv));
-    const bool bf = cache.dtype == KMI_BF16;
-    if (cache.bits == 4) {
+    for (int w = 0; w < 2; ++w) {
+        Side& s = p.side[w];
+        s.rows = w ? p.c.v : p.c.k;
+        s.scales = w ? p.c.vsc : p.c.ksc;
+        for (int i = 0; i < 3; ++i) {
+            s.stride[i] = w ? p.c.vs[i] : p.c.ks[i];
+            s.scale_stride[i] = w ? p.c.vss[i] : p.c.kss[i];
+        }
+        s.out = static_cast<char*>(w ? v : k);
+        s.chunks = (w ? p.c.dv : p.c.d) / 8;
+        s.blocks = static_cast<int>(ceil_div(max_k * s.chunks, THREADS * ITEMS));
+        s.fd_chunks = fwd::fast_div(static_cast<uint32_t>(s.chunks));
+    }
+    const dim3 grid(static_cast<unsigned>((p.side[0].blocks + p.side[1].blocks) * c.batch * c.heads_kv));
+    const bool bf = c.dtype == KMI_BF16;
+    if (c.bits == 4) {
         if (bf)
             hipLaunchKernelGGL((read_kernel<bf16, true>), grid, dim3(THREADS), 0, stream, p);
         else
@@ -762,7 +785,7 @@ bool read_fits(const kmi_paged_cache& c, int64_t max_k) {
     const int64_t per = c.head_dim / 8 + c.head_dim_v / 8;
     if (max_k > ((int64_t{1} << 31) - THREADS * ITEMS) / per) return false;
     const int64_t units = c.batch * c.heads_kv;
-    return units == 0 || ceil_div(max_k * per, THREADS * ITEMS) < (int64_t{1} << 24) / units;
+    return units == 0 || ceil_div(max_k * per, THREADS * ITEMS) + 1 < (int64_t{1} << 24) / units;
 }
 
 }  // namespace paged
