@@ -135,8 +135,7 @@ Plan make_plan(const kmi_paged_attn_args* a) {
 // Nothing is looked up (every split of every row wrote its log-sum-exp), so the first rows are
 // requested beside the sums: one memory round trip.  Rows of empty splits are read and dropped.
 constexpr int MERGE_ROWS = 4;   // of a workgroup
-constexpr int MERGE_BATCH = 8;  // splits in flight
-template <typename T, int DP>
+template <typename T, int DP, int BATCH>  // BATCH: splits in flight
 __global__ __launch_bounds__(MERGE_ROWS * kWave) void merge_kernel(const AttnParams p) {
     constexpr int E = DP <= 64 ? 1 : (DP <= 128 ? 2 : 4);  // dims of a lane (value head dims are multiples of 8)
     const int64_t step = p.rows_total * p.hq;
@@ -147,10 +146,10 @@ __global__ __launch_bounds__(MERGE_ROWS * kWave) void merge_kernel(const AttnPar
         float e[E];
     };
     const float* src = p.part_o + row * DP + dc;
-    Vec x[MERGE_BATCH];
+    Vec x[BATCH];
     auto fetch = [&](int s0) {
 #pragma unroll
-        for (int s = 0; s < MERGE_BATCH; ++s)
+        for (int s = 0; s < BATCH; ++s)
             __builtin_memcpy(&x[s], __builtin_assume_aligned(src + min(s0 + s, p.splits - 1) * step * DP, E * 4), E * 4);
     };
     fetch(0);
@@ -161,10 +160,10 @@ __global__ __launch_bounds__(MERGE_ROWS * kWave) void merge_kernel(const AttnPar
     float acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    for (int s0 = 0; s0 < p.splits; s0 += MERGE_BATCH) {
+    for (int s0 = 0; s0 < p.splits; s0 += BATCH) {
         if (s0 > 0) fetch(s0);
 #pragma unroll
-        for (int s = 0; s < MERGE_BATCH; ++s) {
+        for (int s = 0; s < BATCH; ++s) {
             const float ws = s0 + s < p.splits ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), s0 + s)) : 0.f;
 #pragma unroll
             for (int e = 0; e < E; ++e) acc[e] += ws > 0.f ? ws * x[s].e[e] : 0.f;  // (never written where 0)
@@ -189,8 +188,10 @@ hipError_t run(const AttnParams& p, const Plan& pl, bool four, hipStream_t strea
                                      : launch_tile<T, DP>(p, pl.row_groups, stream);
     if (err != hipSuccess || pl.splits == 1) return err;
     const int64_t rows = p.rows_total * p.hq;
-    hipLaunchKernelGGL((merge_kernel<T, DP>), dim3(static_cast<unsigned>(ceil_div(rows, MERGE_ROWS))),
-                       dim3(MERGE_ROWS * kWave), 0, stream, p);
+    // (Two splits with room for eight read the second seven times: 2 x 777 tokens of 16 x 128 12.0 us,
+    // so 9.7.)
+    hipLaunchKernelGGL((pl.splits == 2 ? merge_kernel<T, DP, 2> : merge_kernel<T, DP, 8>),
+                       dim3(static_cast<unsigned>(ceil_div(rows, MERGE_ROWS))), dim3(MERGE_ROWS * kWave), 0, stream, p);
     return hipGetLastError();
 }
 
