@@ -310,8 +310,8 @@ int kmi_layer_norm_bwd(const void* dy, const void* x, const float* mean, const f
  * each value rounded once.  Two tensors (`x[1]` may be NULL) share the positions and one
  * launch: token (b, s) of [batch, heads, seq, head_dim] tensors, element strides of the
  * batch, head and seq dims, head-dim stride 1.  positions: int32 or int64 (position_bits),
- * element (b, s) at b * position_stride[0] + s * position_stride[1].  y may be x itself
- * with the same strides.  No counterpart among the reference's programs: its fusion covers
+ * element (b, s) at b * position_stride[0] + s * position_stride[1]; fewer than 2^24 tokens.
+ * y may be x itself with the same strides.  No counterpart among the reference's programs: its fusion covers
  * RoPE as a pointwise chain (src/kohakutt/fusion).
  */
 typedef struct kmi_rotary_args {

@@ -86,7 +86,6 @@ std::tuple<Tensor, Tensor> rotary(const Tensor& x_in, const optional<Tensor>& se
                           2 * inv_freq.numel() <= d && inv_freq.device() == x_in.device(),
                       op, "inv_freq must be fp32 [rotated dims / 2], at most ", d / 2, ", on the tensors' device, got ",
                       inv_freq.sizes(), " ", inv_freq.scalar_type());
-    TORCH_CHECK_VALUE(!inv_freq.requires_grad(), op, "inv_freq takes no gradient");
     TORCH_CHECK_VALUE((positions.scalar_type() == at::kLong || positions.scalar_type() == at::kInt) &&
                           positions.device() == x_in.device(),
                       op, "positions must be int32 or int64 on the tensors' device, got ", positions.scalar_type());
@@ -172,6 +171,8 @@ struct RotaryFn : public torch::autograd::Function<RotaryFn> {
 // ktt::_rotary at AutogradCUDA.
 std::tuple<Tensor, Tensor> rotary_autograd(const Tensor& x, const optional<Tensor>& second, const Tensor& positions,
                                            const Tensor& inv_freq, bool interleaved, double scale, bool inverse) {
+    TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !inv_freq.requires_grad(),
+                      "kohakutt_amd.rotary: inv_freq takes no gradient");
     if (at::GradMode::is_enabled() && (x.requires_grad() || (given(second) && second->requires_grad()))) {
         auto out = RotaryFn::apply(x, second, positions, inv_freq, interleaved, scale, inverse);
         return {out[0], out.size() > 1 ? out[1] : Tensor()};
@@ -292,6 +293,8 @@ optional<Tensor> paged_append(const Tensor& k_in, const Tensor& v_in, const Tens
     const Tensor k = rows_operand(k_in), v = rows_operand(v_in);
     Tensor q, q_out, freq;
     if (given(inv_freq)) {
+        TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !inv_freq->requires_grad(), op,
+                          "a cache takes no gradients: call it under torch.no_grad()");
         TORCH_CHECK_VALUE(inv_freq->scalar_type() == at::kFloat && inv_freq->dim() == 1 && inv_freq->numel() >= 1 &&
                               2 * inv_freq->numel() <= a.cache.head_dim && inv_freq->device() == k.device(),
                           op, "inv_freq must be fp32 [rotated dims / 2], at most ", a.cache.head_dim / 2,

@@ -268,6 +268,29 @@ def test_append_leaves_out_what_the_cache_cannot_hold(ops, dev, bits):
     assert out.shape == q.shape and bool((out[sum(new):] == 0).all())
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("interleaved,rd,scale", [(False, 128, 1.0), (True, 128, -0.7), (False, 64, 1.0), (True, 40, 1.0), (False, 24, 1.3)])
+def test_append4_codes_of_many_values(ops, dev, dtype, interleaved, rd, scale):
+    """Three million rotated values, thousands of them within what 32 bits are off of a border
+    between two codes: bit for bit the codes of exact arithmetic."""
+    d, page, heads = 128, 64, 8
+    new, before = [2000, 1000, 7], [5000, 0, 100]
+    if rd < 64:
+        new, before = [90, 40, 7], [3000, 0, 100]
+    c = P.Cache([a + b for a, b in zip(new, before)], heads, d, d, page, dtype, 4, empty=True)
+    held, cu, t = c.to(dev), P.cu_of(new), sum(new)
+    k, v = _randn(t, heads, d, seed=31, dtype=dtype), _randn(t, heads, d, seed=32, dtype=dtype)
+    k[:40] *= 2.0**-60 if dtype is BF else 2.0**-20
+    k[40:60, :, ::7] = 0
+    freq = _freq(rd // 2)
+    ops.paged_append(k.to(dev), v.to(dev), **held, cu_seq=torch.tensor(cu, dtype=torch.int32, device=dev),
+                     inv_freq=freq.to(dev), interleaved=interleaved, rotary_scale=scale)
+    _append_reference(c, k, v, None, cu, freq, interleaved, scale)
+    for name, parts in (("k", c.kt), ("v", c.vt)):
+        assert torch.equal(held[name + "_scale"].cpu(), parts[1])
+        assert torch.equal(held[name + "_cache"].cpu(), parts[0])
+
+
 def test_append4_next_to_borders(ops, dev):
     """Rotated values within 2^-24 of a border between two codes: codes of exact arithmetic."""
     d = 32
@@ -444,6 +467,48 @@ def test_calls_repeat_bit_for_bit_and_sequences_are_independent(ops, dev, bits):
     for new, before in (([1, 1, 1], [900, 41, 300]), ([60, 3, 20], [100, 41, 700])):
         one = _attend(ops, dev, new, before, 2, 4, 128, 128, 32, BF, bits)
         two = _attend(ops, dev, new, before, 2, 4, 128, 128, 32, BF, bits)
+        assert torch.equal(one, two)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("new,before", [([5, 3], [-2, -3]), ([40, 6, 3], [-20, -6, -2]), ([200, 90], [-150, -1])])
+@pytest.mark.parametrize("causal", [True, False])
+def test_more_queries_than_keys(ops, dev, bits, new, before, causal):
+    """The first queries of a sequence see no key (all of them where it holds none)."""
+    _attend(ops, dev, new, before, 2, 4, 64, 64, 16, BF, bits, causal=causal, tail=2)
+
+
+@pytest.mark.parametrize("count", [63, 64, 65, 130])
+def test_many_sequences(ops, dev, count):
+    """Past the sequences that a workgroup sorts by their lengths, single tokens and tiles."""
+    new = [1 + (7 * b) % 41 for b in range(count)]
+    before = [(13 * b) % 90 for b in range(count)]
+    _attend(ops, dev, new, before, 2, 4, 64, 64, 16, BF, 16)
+    _attend(ops, dev, [1] * count, before, 2, 4, 64, 64, 16, BF, 16)
+    _attend(ops, dev, [min(n, 3) for n in new], before, 2, 4, 64, 64, 16, BF, 4)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_sequences_that_share_pages(ops, dev, bits):
+    """A common prefix held once: each sequence reads it as its own, bit for bit."""
+    c = P.Cache([96, 96, 96], 2, 64, 64, 16, BF, bits)
+    held = c.to(dev)
+    pages = held["block_table"]
+    for rows in (1, 3, 30):
+        q = _randn(3 * rows, 8, 64, seed=rows, dtype=BF).to(dev)
+        cu = torch.arange(0, 3 * rows + 1, rows, dtype=torch.int32, device=dev)
+        args = {"cu_seq_q": cu, "max_q": rows, "max_k": 96}
+        shared = pages.clone()
+        shared[1:, :5] = pages[0, :5]
+        copied = {**held}
+        for n in held:
+            if n.endswith(("cache", "scale")):
+                x = held[n].clone()
+                for b in (1, 2):
+                    x[pages[b, :5].long()] = held[n][pages[0, :5].long()]
+                copied[n] = x
+        one = ops.sdpa_paged(q, **{**held, "block_table": shared}, **args)
+        two = ops.sdpa_paged(q, **copied, **args)
         assert torch.equal(one, two)
 
 
@@ -661,3 +726,141 @@ def test_training_step_through_rotary_and_attention(ops, dev):
         # Roundings on the way, one half step (2^-8) each at most: q and k rotated, P, dP's row
         # sums, dS, the gradient, its rotation: independent, so their root sum of squares.
         assert rel <= math.sqrt(8) * 2.0**-8, rel
+
+
+# ---------------------------------------------------------------- refusals
+
+
+def _rotary_call(dev, **kw):
+    args = {
+        "x": torch.zeros(2, 4, 5, 64, dtype=BF, device=dev),
+        "positions": torch.arange(5, device=dev),
+        "inv_freq": torch.ones(32, device=dev),
+        "k": torch.zeros(2, 1, 5, 64, dtype=BF, device=dev),
+    }
+    return {**args, **kw}
+
+
+@pytest.mark.parametrize(
+    "make,msg",
+    [
+        (lambda dev: {"x": torch.zeros(2, 4, 5, 64, dtype=torch.float64, device=dev)}, "bf16, fp16 or fp32"),
+        (lambda dev: {"x": torch.zeros(5, 64, dtype=BF, device=dev)}, "must be"),
+        (lambda dev: {"k": torch.zeros(2, 1, 6, 64, dtype=BF, device=dev)}, "k must match"),
+        (lambda dev: {"k": torch.zeros(2, 1, 5, 64, dtype=HF, device=dev)}, "k must match"),
+        (lambda dev: {"k": torch.zeros(2, 1, 5, 32, dtype=BF, device=dev)}, "k must match"),
+        (lambda dev: {"positions": torch.arange(4, device=dev)}, "positions must be"),
+        (lambda dev: {"positions": torch.zeros(3, 5, dtype=torch.int64, device=dev)}, "positions must be"),
+        (lambda dev: {"positions": torch.zeros(5, device=dev)}, "int32 or int64"),
+        (lambda dev: {"positions": torch.arange(5)}, "int32 or int64 on the tensors' device"),
+        (lambda dev: {"inv_freq": torch.ones(33, device=dev)}, "at most 32"),
+        (lambda dev: {"inv_freq": torch.ones(0, device=dev)}, "at most 32"),
+        (lambda dev: {"inv_freq": torch.ones(32)}, "on the tensors' device"),
+        (lambda dev: {"inv_freq": torch.ones(32, dtype=torch.float64, device=dev)}, "fp32"),
+        (lambda dev: {"inv_freq": torch.ones(32, device=dev, requires_grad=True)}, "no gradient"),
+        (lambda dev: {"inv_freq": torch.ones(32, device=dev, requires_grad=True),
+                      "x": torch.zeros(2, 4, 5, 64, dtype=BF, device=dev, requires_grad=True)}, "no gradient"),
+    ],
+)
+def test_rotary_refuses(ops, dev, make, msg):
+    with pytest.raises((ValueError, RuntimeError), match=msg):
+        ops.rotary(**_rotary_call(dev, **make(dev)))
+
+
+def _cache_calls(dev, bits=16):
+    """Arguments of an append and of an attention call that are accepted."""
+    cache = {n: t for n, t in P.Cache([40, 7], 2, 64, 64, 16, BF, bits).to(dev).items()}
+    k = torch.zeros(2, 2, 64, dtype=BF, device=dev)
+    return cache, {"k": k, "v": k.clone(), **cache}, {"q": torch.zeros(2, 8, 64, dtype=BF, device=dev), **cache}
+
+
+_BAD_CACHES = [
+    (lambda c: {"v_cache": c["v_cache"][1:]}, "must be \\[pages"),
+    (lambda c: {"k_cache": c["k_cache"][0]}, "must be \\[pages"),
+    (lambda c: {"k_cache": c["k_cache"][:, :, :8], "v_cache": c["v_cache"][:, :, :8]}, "multiple of 16"),
+    (lambda c: {"k_cache": c["k_cache"].float()}, "bf16 or fp16"),
+    (lambda c: {"k_cache": c["k_cache"].half(), "v_cache": c["v_cache"].half()}, "not"),
+    (lambda c: {"block_table": c["block_table"].long()}, "block_table must be int32"),
+    (lambda c: {"block_table": c["block_table"][0]}, "block_table must be int32"),
+    (lambda c: {"block_table": c["block_table"].cpu()}, "on one device"),
+    (lambda c: {"block_table": c["block_table"].t().contiguous().t()}, "rows must be contiguous"),
+    (lambda c: {"key_lengths": c["key_lengths"].long()}, "key_lengths must be int32"),
+    (lambda c: {"key_lengths": c["key_lengths"][:1]}, "key_lengths must be int32"),
+    (lambda c: {"k_cache": c["k_cache"].transpose(2, 3).contiguous().transpose(2, 3)}, "contiguous"),
+    (lambda c: {"k_scale": c["k_cache"].to(torch.uint8)}, "four uint8 tensors"),
+]
+
+
+@pytest.mark.parametrize("make,msg", _BAD_CACHES)
+def test_bad_caches_are_refused(ops, dev, make, msg):
+    cache, append, attend = _cache_calls(dev)
+    bad = make(cache)
+    with pytest.raises((ValueError, RuntimeError), match=msg):
+        ops.paged_append(**{**append, **bad})
+    with pytest.raises((ValueError, RuntimeError), match=msg):
+        ops.sdpa_paged(**{**attend, **bad})
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize(
+    "make,msg",
+    [
+        (lambda a, dev: {"k": a["k"][:1]}, "must be \\[T, heads, D\\]"),
+        (lambda a, dev: {"k": a["k"][:, :, :32], "v": a["v"]}, "the cache holds"),
+        (lambda a, dev: {"k": a["k"][:, :1], "v": a["v"][:, :1]}, "the cache holds"),
+        (lambda a, dev: {"k": a["k"].half()}, "one type"),
+        (lambda a, dev: {"k": a["k"].repeat(2, 1, 1), "v": a["v"].repeat(2, 1, 1)}, "one token per sequence"),
+        (lambda a, dev: {"cu_seq": torch.tensor([0, 2], dtype=torch.int32, device=dev)}, "offsets must be"),
+        (lambda a, dev: {"cu_seq": torch.tensor([0, 1, 2], device=dev)}, "offsets must be"),
+        (lambda a, dev: {"cu_seq": torch.tensor([0, 1, 2], dtype=torch.int32)}, "offsets must be"),
+        (lambda a, dev: {"q": torch.zeros(2, 8, 64, dtype=BF, device=dev)}, "needs inv_freq"),
+        (lambda a, dev: {"q": torch.zeros(3, 8, 64, dtype=BF, device=dev), "inv_freq": torch.ones(32, device=dev)}, "q must be"),
+        (lambda a, dev: {"inv_freq": torch.ones(40, device=dev)}, "at most 32"),
+        (lambda a, dev: {"inv_freq": torch.ones(32, device=dev, requires_grad=True)}, "no_grad"),
+        (lambda a, dev: {"k": a["k"].clone().requires_grad_()}, "no_grad"),
+    ],
+)
+def test_append_refuses(ops, dev, bits, make, msg):
+    _, append, _ = _cache_calls(dev, bits)
+    with pytest.raises((ValueError, RuntimeError), match=msg):
+        ops.paged_append(**{**append, **make(append, dev)})
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize(
+    "make,msg",
+    [
+        (lambda a, dev: {"q": a["q"].float()}, "bf16 or fp16"),
+        (lambda a, dev: {"q": a["q"][0]}, "q must be"),
+        (lambda a, dev: {"q": a["q"][:, :7]}, "must divide"),
+        (lambda a, dev: {"q": a["q"][:, :, :32].contiguous()}, "the cache holds"),
+        (lambda a, dev: {"q": a["q"].repeat(2, 1, 1)}, "one token per sequence"),
+        (lambda a, dev: {"max_q": -1}, "not be negative"),
+        (lambda a, dev: {"max_k": -1}, "not be negative"),
+        (lambda a, dev: {"q": a["q"].clone().requires_grad_()}, "no_grad"),
+        (lambda a, dev: {"cu_seq_q": torch.tensor([0, 2], dtype=torch.int32, device=dev)}, "offsets must be"),
+    ],
+)
+def test_attention_refuses(ops, dev, bits, make, msg):
+    _, _, attend = _cache_calls(dev, bits)
+    with pytest.raises((ValueError, RuntimeError), match=msg):
+        ops.sdpa_paged(**{**attend, **make(attend, dev)})
+
+
+def test_four_bit_gaps_are_refused(ops, dev):
+    cache, append, attend = _cache_calls(dev, 4)
+    for bad, msg in (
+        ({"v_scale": None}, "four uint8 tensors"),
+        ({"k_scale": cache["k_scale"].to(torch.int8)}, "four uint8 tensors"),
+        ({"k_scale": cache["k_scale"][..., :1]}, "scales must be"),
+        ({"k_scale": cache["k_scale"].cpu()}, "scales must be"),
+        ({"k_cache": cache["k_cache"][..., :24], "v_cache": cache["v_cache"][..., :24]}, "scales must be"),
+    ):
+        with pytest.raises((ValueError, RuntimeError), match=msg):
+            ops.paged_append(**{**append, **bad})
+        with pytest.raises((ValueError, RuntimeError), match=msg):
+            ops.sdpa_paged(**{**attend, **bad})
+    with pytest.raises((ValueError, RuntimeError), match="max_k"):
+        ops.paged_read(**cache, max_k=-1)
+    with pytest.raises((ValueError, RuntimeError), match="bf16 or fp16"):
+        ops.paged_read(**cache, max_k=4, dtype=torch.float32)
