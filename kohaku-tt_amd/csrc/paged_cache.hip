@@ -275,14 +275,17 @@ __global__ __launch_bounds__(THREADS) void append_kernel(const AppendParams p) {
     struct Vec {
         T e[VW];
     };
-    auto first_dim = [&](int c) { return c < nrot ? (INTER ? 2 * VW * c : VW * c) : p.rd + VW * (c - nrot); };
+    // A pair of vectors is one of each half of the rotated dims in either layout, so that a
+    // wavefront's loads are of one piece (as in rotary.hip).
+    constexpr bool NEXT = INTER && VW == 1;
+    auto first_dim = [&](int c) { return c < nrot ? (NEXT ? 2 * c : VW * c) : p.rd + VW * (c - nrot); };
     auto load = [&](const T* from) {
         Vec v;
         __builtin_memcpy(&v, __builtin_assume_aligned(from, VW * 2), VW * 2);
         return v;
     };
     auto store = [&](T* to, const Vec& v) { __builtin_memcpy(__builtin_assume_aligned(to, VW * 2), &v, VW * 2); };
-    const int apart = INTER ? VW : half;
+    const int apart = NEXT ? 1 : half;
     Vec a[ITEMS], z[ITEMS];
     auto fetch = [&](int base) {
 #pragma unroll
@@ -319,8 +322,18 @@ __global__ __launch_bounds__(THREADS) void append_kernel(const AppendParams p) {
                 continue;
             }
             float cs[VW], sn[VW];
-            __builtin_memcpy(cs, __builtin_assume_aligned(cosine + m.tl * half + VW * m.c, VW * 4), VW * 4);
-            __builtin_memcpy(sn, __builtin_assume_aligned(sine + m.tl * half + VW * m.c, VW * 4), VW * 4);
+            if constexpr (INTER && VW > 1) {
+                // (Pairs lie within a vector: the angles of the two are half of all apart.)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int k = m.tl * half + VW / 2 * m.c + i * (half / 2);
+                    __builtin_memcpy(cs + i * (VW / 2), __builtin_assume_aligned(cosine + k, VW * 2), VW * 2);
+                    __builtin_memcpy(sn + i * (VW / 2), __builtin_assume_aligned(sine + k, VW * 2), VW * 2);
+                }
+            } else {
+                __builtin_memcpy(cs, __builtin_assume_aligned(cosine + m.tl * half + VW * m.c, VW * 4), VW * 4);
+                __builtin_memcpy(sn, __builtin_assume_aligned(sine + m.tl * half + VW * m.c, VW * 4), VW * 4);
+            }
             Vec u, w;
             auto pair = [&](T p1, T p2, int e, T& y1, T& y2) {
                 float f1, f2;

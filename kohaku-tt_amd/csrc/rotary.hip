@@ -2,14 +2,16 @@
 // inv_freq, forward and (by the opposite angle) backward.
 //
 // Bound by memory: every value is read and written once, for three operations.  A workgroup owns
-// a few tokens.  Its threads first request their vectors (a pair of 16-byte vectors of one head
-// each: one of each half, or two adjacent ones when interleaved), then form the tokens' sines and
-// cosines into LDS, one pair a thread (about 45 instructions, the angles in 64 bits, behind the
-// loads' latency), and then turn and store.  Angles are so formed once per token and not per
-// head, and no thread walks the heads one after the other.
+// a few tokens.  Its threads first request their vectors (two of 16 bytes each, one of each half of
+// a head's rotated dims), then form the tokens' sines and cosines into LDS, one pair a thread (about
+// 45 instructions, the angles in 64 bits, behind the loads' latency), and then turn and store.
+// Angles are so formed once per token and not per head, and no thread walks the heads one after the
+// other.  Interleaved pairs lie within a vector; two adjacent vectors a thread, which leave gaps
+// between a wavefront's lanes, took 43.8 us where the halves take 40.5.
 //
-// Measured: 4 x 4096 tokens of 16 and 8 heads x 128 (201 MB) 43.5 us, 4.6 TB/s (a large copy moves
-// 5.1), of 8 tokens 3.3 us (one memory round trip behind the launch; a call's host path is 7).
+// Measured: 4 x 4096 tokens of 16 and 8 heads x 128 (201 MB) 39.0 us, 5.2 TB/s (a large copy moves
+// 5.1), interleaved 40.5; 8 tokens 2.8 us, one memory round trip behind the launch (the host's part
+// of a call is 7).
 #include <algorithm>
 
 #include "paged.hpp"
@@ -88,9 +90,9 @@ __global__ __launch_bounds__(THREADS) void rotary_kernel(const Params p) {
             const T* x = static_cast<const T*>(p.x[w]) + b * p.xs[w][0] + h * p.xs[w][1] + s * p.xs[w][2];
             dst[j] = static_cast<T*>(p.y[w]) + b * p.ys[w][0] + h * p.ys[w][1] + s * p.ys[w][2];
             const bool rot = c < nrot;
-            lo[j] = rot ? (INTER ? 2 * V * c : V * c) : p.rd + V * (c - nrot);
-            hi[j] = INTER ? lo[j] + V : lo[j] + half;
-            at[j] = rot ? tl * half + V * c : -1;
+            lo[j] = rot ? (INTER && V == 1 ? 2 * c : V * c) : p.rd + V * (c - nrot);
+            hi[j] = INTER && V == 1 ? lo[j] + 1 : lo[j] + half;
+            at[j] = rot ? tl * half + (INTER && V > 1 ? V / 2 : V) * c : -1;
             a[j] = load<T, V>(x + lo[j]);
             if (rot) z[j] = load<T, V>(x + hi[j]);
         }
@@ -117,8 +119,18 @@ __global__ __launch_bounds__(THREADS) void rotary_kernel(const Params p) {
                 continue;
             }
             float cs[V], sn[V];
-            __builtin_memcpy(cs, __builtin_assume_aligned(cosine + at[j], V * 4), V * 4);
-            __builtin_memcpy(sn, __builtin_assume_aligned(sine + at[j], V * 4), V * 4);
+            if constexpr (INTER && V > 1) {
+                // Pairs lie within a vector: the angles of the two vectors are half of all apart.
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int k = at[j] + i * (half / 2);
+                    __builtin_memcpy(cs + i * (V / 2), __builtin_assume_aligned(cosine + k, V * 2), V * 2);
+                    __builtin_memcpy(sn + i * (V / 2), __builtin_assume_aligned(sine + k, V * 2), V * 2);
+                }
+            } else {
+                __builtin_memcpy(cs, __builtin_assume_aligned(cosine + at[j], V * 4), V * 4);
+                __builtin_memcpy(sn, __builtin_assume_aligned(sine + at[j], V * 4), V * 4);
+            }
             Vec<T, V> u, w;
             if constexpr (INTER && V > 1) {
 #pragma unroll
