@@ -399,7 +399,7 @@ def _attend(ops, dev, new, before, heads, group, d, dv, page, dtype, bits, causa
     "keys,heads,group,d,page",
     [([1], 1, 1, 64, 16), ([16, 17, 31, 32, 33], 2, 8, 128, 16), ([777], 2, 7, 64, 16), ([0, 5, 0], 1, 4, 128, 64),
      ([1000, 3, 129, 128], 3, 5, 96, 48), ([2500, 40], 1, 16, 256, 128), ([90, 300], 2, 32, 64, 32),
-     ([600], 1, 17, 128, 256), ([4097], 1, 1, 32, 64), ([130, 61], 2, 3, 192, 16)],
+     ([600], 1, 17, 128, 256), ([4097], 1, 1, 32, 64), ([130, 61], 2, 3, 192, 16), ([300, 0, 5], 1, 48, 64, 32)],
 )
 def test_single_tokens(ops, dev, bits, dtype, keys, heads, group, d, page):
     _attend(ops, dev, [1] * len(keys), [n - 1 for n in keys], heads, group, d, d, page, dtype, bits)
