@@ -112,6 +112,14 @@ __device__ __forceinline__ void turned(float x1, float x2, float c, float s, flo
     y2 = __builtin_fmaf(x2, c, x1 * s);
 }
 
+// Inputs that a kernel reads once are read past the caches (non-temporal loads) from this size on, a
+// quarter of the last-level cache: the results then stay there instead.  Measured on the rotation
+// (us, through the caches / past them; after the product that writes its input): 25 MB 9.7 / 10.2
+// (19.5 / 19.4), 50 MB 18.6 / 21.1 (34.1 / 34.1), 75 MB 30.1 / 30.6 (51.1 / 50.6), 101 MB 39.6 / 38.3
+// (68.4 / 66.0), 201 MB 77.9 / 67.1 (144.7 / 136.8).  Results written past them cost what reads
+// them next more than they save (201 MB 78.0 / 73.3, with a sum over them 119.4 / 126.7).
+constexpr int64_t kStreamBytes = int64_t{64} << 20;
+
 // ---------------------------------------------------------------- 4 bits
 
 // Two of the values a dword of eight codes stands for (codes 2 sel and 2 sel + 1) times the

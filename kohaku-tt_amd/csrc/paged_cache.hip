@@ -229,7 +229,7 @@ using V8 = typename Vec8<T>::type;
 // ---------------------------------------------------------------- 16 bits
 
 // A workgroup of values: `out` stores a chunk of eight dims at its place.
-template <typename T, typename F>
+template <typename T, bool STREAM, typename F>
 __device__ __forceinline__ void append_values(const AppendParams& p, int block, Held* held, F out) {
     const int t0 = block * p.tpb_v;
     const int nt = min(p.tpb_v, p.c.tokens - t0);
@@ -241,8 +241,9 @@ __device__ __forceinline__ void append_values(const AppendParams& p, int block, 
             const int i = base + j * THREADS + threadIdx.x;
             if (i >= items) continue;
             const Item m = v_item(p, i);
-            x[j] = *reinterpret_cast<const V8<T>*>(static_cast<const T*>(p.v) + static_cast<int64_t>(t0 + m.tl) * p.vs[0] +
-                                                   m.h * p.vs[1] + 8 * m.c);
+            const V8<T>* const src = reinterpret_cast<const V8<T>*>(
+                static_cast<const T*>(p.v) + static_cast<int64_t>(t0 + m.tl) * p.vs[0] + m.h * p.vs[1] + 8 * m.c);
+            x[j] = STREAM ? __builtin_nontemporal_load(src) : *src;
         }
         if (base == 0) place_tokens<float>(p, p.c.vs, p.c.vss, t0, nt, held, nullptr, nullptr);
 #pragma unroll
@@ -258,12 +259,12 @@ __device__ __forceinline__ void append_values(const AppendParams& p, int block, 
 
 // Query and key chunks of VW dims a half: both vectors of a rotated pair in one thread.  VW is 8,
 // or 1 where the rotated dims are no whole pairs of vectors.
-template <typename T, int VW, bool INTER>
+template <typename T, int VW, bool INTER, bool STREAM>
 __global__ __launch_bounds__(THREADS) void append_kernel(const AppendParams p) {
     __shared__ __align__(16) float cosine[PAIRS], sine[PAIRS];
     __shared__ Held held[TOKENS];
     if (static_cast<int>(blockIdx.x) >= p.blocks_qk) {
-        append_values<T>(p, blockIdx.x - p.blocks_qk, held, [&](const Held& at, int h, int c, const V8<T>& x) {
+        append_values<T, STREAM>(p, blockIdx.x - p.blocks_qk, held, [&](const Held& at, int h, int c, const V8<T>& x) {
             *reinterpret_cast<V8<T>*>(v_place(p, at, h) + 16 * c) = x;
         });
         return;
@@ -281,7 +282,10 @@ __global__ __launch_bounds__(THREADS) void append_kernel(const AppendParams p) {
     auto first_dim = [&](int c) { return c < nrot ? (NEXT ? 2 * c : VW * c) : p.rd + VW * (c - nrot); };
     auto load = [&](const T* from) {
         Vec v;
-        __builtin_memcpy(&v, __builtin_assume_aligned(from, VW * 2), VW * 2);
+        if constexpr (STREAM && VW == 8)
+            v = __builtin_bit_cast(Vec, __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(from)));
+        else
+            __builtin_memcpy(&v, __builtin_assume_aligned(from, VW * 2), VW * 2);
         return v;
     };
     auto store = [&](T* to, const Vec& v) { __builtin_memcpy(__builtin_assume_aligned(to, VW * 2), &v, VW * 2); };
@@ -474,7 +478,7 @@ __global__ __launch_bounds__(THREADS) void append4_kernel(const AppendParams p) 
     __shared__ Held held[TOKENS];
     typedef V8<T> v8;
     if (static_cast<int>(blockIdx.x) >= p.blocks_qk) {
-        append_values<T>(p, blockIdx.x - p.blocks_qk, held, [&](const Held& at, int h, int c, const v8& x) {
+        append_values<T, false>(p, blockIdx.x - p.blocks_qk, held, [&](const Held& at, int h, int c, const v8& x) {
             int byte;
             *reinterpret_cast<uint32_t*>(v_place(p, at, h) + 4 * c) = quantise<T>(x, byte);
             if ((c & 3) == 0) p.c.vsc[at.scale + h * p.c.vss[1] + (c >> 2)] = static_cast<uint8_t>(byte);
@@ -669,10 +673,12 @@ hipError_t launch_append(const kmi_paged_append_args* a, hipStream_t stream) {
     auto enqueue = [&](void (*kernel)(AppendParams)) { hipLaunchKernelGGL(kernel, grid, dim3(THREADS), 0, stream, p); };
     if (four)
         enqueue(p.inter ? append4_kernel<T, true> : append4_kernel<T, false>);
+    else if (vw == 8 && tokens * (static_cast<int64_t>(p.hq + p.c.hkv) * p.c.d + p.c.hkv * p.c.dv) * 2 >= kStreamBytes)
+        enqueue(p.inter ? append_kernel<T, 8, true, true> : append_kernel<T, 8, false, true>);
     else if (vw == 8)
-        enqueue(p.inter ? append_kernel<T, 8, true> : append_kernel<T, 8, false>);
+        enqueue(p.inter ? append_kernel<T, 8, true, false> : append_kernel<T, 8, false, false>);
     else
-        enqueue(p.inter ? append_kernel<T, 1, true> : append_kernel<T, 1, false>);
+        enqueue(p.inter ? append_kernel<T, 1, true, false> : append_kernel<T, 1, false, false>);
     return hipGetLastError();
 }
 

@@ -44,11 +44,13 @@ struct Vec {
     T e[V];
 };
 
-template <typename T, int V>
+template <typename T, int V, bool STREAM>
 __device__ __forceinline__ Vec<T, V> load(const T* p) {
     Vec<T, V> v;
     if constexpr (V == 1)
         v.e[0] = *p;
+    else if constexpr (STREAM)
+        v = __builtin_bit_cast(Vec<T, V>, __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)));
     else
         __builtin_memcpy(&v, __builtin_assume_aligned(p, 16), 16);
     return v;
@@ -65,7 +67,7 @@ constexpr int THREADS = 256;
 constexpr int ITEMS = 4;       // of a thread, in flight together
 constexpr int PAIRS = 2048;    // angles of a workgroup
 
-template <typename T, int V, bool INTER>
+template <typename T, int V, bool INTER, bool STREAM>
 __global__ __launch_bounds__(THREADS) void rotary_kernel(const Params p) {
     __shared__ __align__(16) float cosine[PAIRS], sine[PAIRS];
     const int t0 = blockIdx.x * p.tpb;
@@ -93,8 +95,8 @@ __global__ __launch_bounds__(THREADS) void rotary_kernel(const Params p) {
             lo[j] = rot ? (INTER && V == 1 ? 2 * c : V * c) : p.rd + V * (c - nrot);
             hi[j] = INTER && V == 1 ? lo[j] + 1 : lo[j] + half;
             at[j] = rot ? tl * half + (INTER && V > 1 ? V / 2 : V) * c : -1;
-            a[j] = load<T, V>(x + lo[j]);
-            if (rot) z[j] = load<T, V>(x + hi[j]);
+            a[j] = load<T, V, STREAM>(x + lo[j]);
+            if (rot) z[j] = load<T, V, STREAM>(x + hi[j]);
         }
     };
     fetch(0);
@@ -216,16 +218,14 @@ hipError_t launch(const kmi_rotary_args* a, hipStream_t stream) {
     p.fd_chunks = fwd::fast_div(static_cast<uint32_t>(p.chunks));
     p.fd_per = fwd::fast_div(static_cast<uint32_t>(p.per));
     const dim3 grid(static_cast<unsigned>(ceil_div(p.tokens, p.tpb)));
-    if (vec) {
-        if (a->interleaved)
-            hipLaunchKernelGGL((rotary_kernel<T, W, true>), grid, dim3(THREADS), 0, stream, p);
-        else
-            hipLaunchKernelGGL((rotary_kernel<T, W, false>), grid, dim3(THREADS), 0, stream, p);
-    } else if (a->interleaved) {
-        hipLaunchKernelGGL((rotary_kernel<T, 1, true>), grid, dim3(THREADS), 0, stream, p);
-    } else {
-        hipLaunchKernelGGL((rotary_kernel<T, 1, false>), grid, dim3(THREADS), 0, stream, p);
-    }
+    const bool past = p.tokens * (p.heads[0] + p.heads[1]) * p.d * static_cast<int64_t>(sizeof(T)) >= paged::kStreamBytes;
+    auto enqueue = [&](void (*kernel)(Params)) { hipLaunchKernelGGL(kernel, grid, dim3(THREADS), 0, stream, p); };
+    if (vec && past)
+        enqueue(a->interleaved ? rotary_kernel<T, W, true, true> : rotary_kernel<T, W, false, true>);
+    else if (vec)
+        enqueue(a->interleaved ? rotary_kernel<T, W, true, false> : rotary_kernel<T, W, false, false>);
+    else
+        enqueue(a->interleaved ? rotary_kernel<T, 1, true, false> : rotary_kernel<T, 1, false, false>);
     return hipGetLastError();
 }
 

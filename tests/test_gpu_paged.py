@@ -268,6 +268,39 @@ def test_append_leaves_out_what_the_cache_cannot_hold(ops, dev, bits):
     assert out.shape == q.shape and bool((out[sum(new):] == 0).all())
 
 
+@pytest.mark.parametrize("dtype,interleaved", [(BF, False), (HF, True), (FP, True)])
+def test_large_inputs_as_their_parts(ops, dev, dtype, interleaved):
+    """64 MB of inputs and more are read past the caches: bit for bit what their parts give."""
+    tokens, heads, d, rd = 5000, 56 if dtype is FP else 64, 128, 96
+    x = torch.randn(tokens, heads, d, device=dev).to(dtype)
+    freq, pos = _freq(rd // 2).to(dev), torch.arange(tokens, device=dev) * 3
+    assert x.numel() * x.element_size() >= 2**26
+    whole = ops.rotary(x, pos, freq, interleaved=interleaved)
+    part = torch.cat([ops.rotary(a, b, freq, interleaved=interleaved) for a, b in zip(x.split(1250), pos.split(1250))])
+    assert torch.equal(whole, part)
+    _check_rotated(whole[:40], x[:40].cpu(), pos[:40].cpu().unsqueeze(1), freq.cpu(), interleaved)
+    if dtype is FP:
+        return
+    k, v, q = x[:, :16], x[:, 16:32], x[:, 32:]
+    cache = [ops.paged_cache(tokens // 50, 16, 64, d, dtype=dtype, device=dev) for _ in range(2)]
+    table = torch.arange(tokens // 50, dtype=torch.int32, device=dev).unsqueeze(0)
+
+    def call(held, lo, hi):
+        cu = torch.tensor([0, hi - lo], dtype=torch.int32, device=dev)
+        return ops.paged_append(k[lo:hi], v[lo:hi], **held, block_table=table, key_lengths=cu[1:], cu_seq=cu, q=q[lo:hi],
+                                inv_freq=freq, interleaved=interleaved)
+
+    one = call(cache[0], 0, tokens)
+    # (The second part's tokens are keys 2500 .. of the sequence.)
+    first = call(cache[1], 0, 2500)
+    cu = torch.tensor([0, 2500], dtype=torch.int32, device=dev)
+    second = ops.paged_append(k[2500:], v[2500:], **cache[1], block_table=table, cu_seq=cu, q=q[2500:], inv_freq=freq,
+                              key_lengths=torch.tensor([tokens], dtype=torch.int32, device=dev), interleaved=interleaved)
+    assert torch.equal(one, torch.cat((first, second)))
+    for n in ("k_cache", "v_cache"):
+        assert torch.equal(cache[0][n], cache[1][n])
+
+
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("interleaved,rd,scale", [(False, 128, 1.0), (True, 128, -0.7), (False, 64, 1.0), (True, 40, 1.0), (False, 24, 1.3)])
 def test_append4_codes_of_many_values(ops, dev, dtype, interleaved, rd, scale):
