@@ -4,8 +4,8 @@
 // values, find the tokens' places (one thread a token) and form their sines and cosines into LDS
 // behind those loads' latency, and then turn, quantise and store, so that nothing waits for a
 // token's chain of lengths, table entry and angle but the stores.  16-bit rows move as 16-byte
-// vectors (bound by memory: 8 x up to 2048 tokens of 16/8 heads x 128, 182 MB, 43.5 us, 4.2 TB/s;
-// 64 single tokens 3.5 us).  A 4-bit row's groups of 32 dims lie in four neighbouring lanes, eight
+// vectors (bound by memory: 8 x up to 2048 tokens of 16/8 heads x 128, 182 MB, 39.2 us, 4.6 TB/s;
+// 64 single tokens 3.6 us).  A 4-bit row's groups of 32 dims lie in four neighbouring lanes, eight
 // dims each, which agree on the group's exponent by two lane exchanges.  A value that 32 bits put on
 // the wrong side of a border between two codes would come out a whole step off, so codes are those
 // of exact arithmetic: keys are rotated in 32 bits, and once more in 64 where one of a group lies

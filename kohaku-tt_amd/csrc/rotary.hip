@@ -7,10 +7,10 @@
 // 45 instructions, the angles in 64 bits, behind the loads' latency), and then turn and store.
 // Angles are so formed once per token and not per head, and no thread walks the heads one after the
 // other.  Interleaved pairs lie within a vector; two adjacent vectors a thread, which leave gaps
-// between a wavefront's lanes, took 43.8 us where the halves take 40.5.
+// between a wavefront's lanes, took 43.8 us where the halves took 40.5.
 //
-// Measured: 4 x 4096 tokens of 16 and 8 heads x 128 (201 MB) 39.0 us, 5.2 TB/s (a large copy moves
-// 5.1), interleaved 40.5; 8 tokens 2.8 us, one memory round trip behind the launch (the host's part
+// Measured: 4 x 4096 tokens of 16 and 8 heads x 128 (201 MB) 38.0 us, 5.3 TB/s (a large copy moves
+// 5.1), interleaved 39.2; 8 tokens 2.8 us, one memory round trip behind the launch (the host's part
 // of a call is 7).
 #include <algorithm>
 
