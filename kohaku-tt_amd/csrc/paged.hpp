@@ -150,9 +150,10 @@ __device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_floa
 // Why a cache is refused, or null.  writes: an append (k / v are written).
 const char* check_cache(const kmi_paged_cache& c, bool uses_tokens);
 Cache device_cache(const kmi_paged_cache& c);
-// Whether a dense copy of max_k keys a sequence can be launched, and the launch (kmi_paged_read).
+// Whether a dense copy of max_k keys a sequence can be launched, and the launch (kmi_paged_read;
+// end: rows past a sequence's length are zeroed and not left out).
 bool read_fits(const kmi_paged_cache& c, int64_t max_k);
-hipError_t launch_read(const kmi_paged_cache& c, void* k, void* v, int64_t max_k, hipStream_t stream);
+hipError_t launch_read(const kmi_paged_cache& c, void* k, void* v, int64_t max_k, bool end, hipStream_t stream);
 
 }  // namespace paged
 }  // namespace kmi

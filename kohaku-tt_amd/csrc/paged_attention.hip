@@ -131,52 +131,58 @@ Plan make_plan(const kmi_paged_attn_args* a) {
     return pl;
 }
 
-// One wavefront per (query token, query head): the splits' normalised rows weighted by their sums.
-// Nothing is looked up (every split of every row wrote its log-sum-exp), so the first rows are
-// requested beside the sums: one memory round trip.  Rows of empty splits are read and dropped.
-constexpr int MERGE_ROWS = 4;   // of a workgroup
-template <typename T, int DP, int BATCH>  // BATCH: splits in flight
-__global__ __launch_bounds__(MERGE_ROWS * kWave) void merge_kernel(const AttnParams p) {
-    constexpr int E = DP <= 64 ? 1 : (DP <= 128 ? 2 : 4);  // dims of a lane (value head dims are multiples of 8)
+// The splits' normalised rows weighted by their sums, a (query token, query head) to as many lanes as
+// it has vectors of four dims.  Nothing is looked up (every split of every row wrote its
+// log-sum-exp), so the first rows are requested beside the sums: one memory round trip.  Rows of
+// empty splits are read and dropped.  2 x 777 tokens of 16 x 128 in two splits (26 MB) 6.8 us; a
+// wavefront a row with two dims a lane 9.7, with room for eight splits 12.0 (BATCH: in flight).
+constexpr int merge_lanes(int dp) { return dp <= 32 ? 8 : dp <= 64 ? 16 : dp <= 128 ? 32 : 64; }
+constexpr int MERGE_THREADS = 256;
+template <typename T, int DP, int BATCH>
+__global__ __launch_bounds__(MERGE_THREADS) void merge_kernel(const AttnParams p) {
+    constexpr int LANES = merge_lanes(DP), ROWS = MERGE_THREADS / LANES;
     const int64_t step = p.rows_total * p.hq;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * MERGE_ROWS + (threadIdx.x >> 6);
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / LANES;
     if (row >= step) return;
-    const int lane = threadIdx.x & 63, d0 = lane * E, dc = min(d0, p.dv - E);
-    struct Vec {
-        float e[E];
-    };
-    const float* src = p.part_o + row * DP + dc;
-    Vec x[BATCH];
-    auto fetch = [&](int s0) {
-#pragma unroll
-        for (int s = 0; s < BATCH; ++s)
-            __builtin_memcpy(&x[s], __builtin_assume_aligned(src + min(s0 + s, p.splits - 1) * step * DP, E * 4), E * 4);
-    };
-    fetch(0);
-    const float lse = lane < p.splits ? p.part_lse[lane * step + row] : -INFINITY;
-    const float top = wave_max(lse);
-    const float w = lse == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(lse - top);
-    const float total = wave_sum(w);
-    float acc[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    const int lane = threadIdx.x % LANES, d0 = 4 * lane;
+    const float* const src = p.part_o + row * DP + min(d0, p.dv - 4);
+    float top = -INFINITY, total = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     for (int s0 = 0; s0 < p.splits; s0 += BATCH) {
-        if (s0 > 0) fetch(s0);
+        f32x4 x[BATCH];
+        float lse[BATCH];
 #pragma unroll
         for (int s = 0; s < BATCH; ++s) {
-            const float ws = s0 + s < p.splits ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), s0 + s)) : 0.f;
+            const int64_t at = min(s0 + s, p.splits - 1) * step;
+            x[s] = *reinterpret_cast<const f32x4*>(src + at * DP);
+            lse[s] = p.part_lse[at + row];
+        }
+        float most = top;
 #pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] += ws > 0.f ? ws * x[s].e[e] : 0.f;  // (never written where 0)
+        for (int s = 0; s < BATCH; ++s) {
+            if (s0 + s >= p.splits) lse[s] = -INFINITY;
+            most = fmaxf(most, lse[s]);
+        }
+        const float shrink = most == top ? 1.f : __builtin_amdgcn_exp2f(top - most);
+        acc *= shrink;
+        total *= shrink;
+        top = most;
+#pragma unroll
+        for (int s = 0; s < BATCH; ++s) {
+            const float w = lse[s] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(lse[s] - top);
+            total += w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] += w > 0.f ? w * x[s][e] : 0.f;  // (never written where 0)
         }
     }
     const int tok = static_cast<int>(row / p.hq), head = static_cast<int>(row - static_cast<int64_t>(tok) * p.hq);
     if (d0 < p.dv) {
         const float inv = total == 0.f ? 0.f : 1.f / total;
-        T y[E];
+        typedef T t4 __attribute__((ext_vector_type(4)));
+        t4 y;
 #pragma unroll
-        for (int e = 0; e < E; ++e) y[e] = from_f32<T>(acc[e] * inv);
-        T* dst = static_cast<T*>(p.out) + head * p.os[1] + tok * p.os[2] + d0;
-        __builtin_memcpy(__builtin_assume_aligned(dst, E * 2), y, E * 2);
+        for (int e = 0; e < 4; ++e) y[e] = from_f32<T>(acc[e] * inv);
+        *reinterpret_cast<t4*>(static_cast<T*>(p.out) + head * p.os[1] + tok * p.os[2] + d0) = y;
     }
     if (p.lse && lane == 0)
         p.lse[head * p.ls[1] + tok * p.ls[2]] = total == 0.f ? -INFINITY : (top + log2f(total)) * 0.6931471805599453f;
@@ -188,10 +194,9 @@ hipError_t run(const AttnParams& p, const Plan& pl, bool four, hipStream_t strea
                                      : launch_tile<T, DP>(p, pl.row_groups, stream);
     if (err != hipSuccess || pl.splits == 1) return err;
     const int64_t rows = p.rows_total * p.hq;
-    // (Two splits with room for eight read the second seven times: 2 x 777 tokens of 16 x 128 12.0 us,
-    // so 9.7.)
     hipLaunchKernelGGL((pl.splits == 2 ? merge_kernel<T, DP, 2> : merge_kernel<T, DP, 8>),
-                       dim3(static_cast<unsigned>(ceil_div(rows, MERGE_ROWS))), dim3(MERGE_ROWS * kWave), 0, stream, p);
+                       dim3(static_cast<unsigned>(ceil_div(rows, MERGE_THREADS / merge_lanes(DP)))), dim3(MERGE_THREADS), 0,
+                       stream, p);
     return hipGetLastError();
 }
 
@@ -273,7 +278,7 @@ extern "C" int kmi_paged_attn(const kmi_paged_attn_args* a, void* workspace, siz
         const int64_t units = a->cache.batch * a->cache.heads_kv;
         char* const kc = static_cast<char*>(workspace);
         char* const vc = kc + static_cast<size_t>(units) * keys * a->cache.head_dim * 2;
-        const hipError_t err = launch_read(a->cache, kc, vc, keys, s);
+        const hipError_t err = launch_read(a->cache, kc, vc, keys, false, s);
         if (err != hipSuccess) return hip_status(err, "kmi_paged_attn");
         p.head_pages = 1;
         p.c.k = kc;

@@ -699,6 +699,7 @@ struct ReadParams {
     Cache c;
     Side side[2];
     int max_k;
+    int end;  // 1: rows past a sequence's length are zeroed, 0: left out
 };
 
 // A workgroup copies chunks of one unit's keys or values.
@@ -713,6 +714,8 @@ __global__ __launch_bounds__(THREADS) void read_kernel(const ReadParams p) {
     if (values) block -= p.side[0].blocks;
     const int first = block * (THREADS * ITEMS) + threadIdx.x;
     const int lk = min(max(uniform_i32(p.c.klen + b), 0), p.c.capacity);
+    const int rows_out = p.end ? p.max_k : min(lk, p.max_k);
+    if (fwd::fdiv(block * (THREADS * ITEMS), side.fd_chunks) >= rows_out) return;
     u32x4 x[ITEMS];
     uint32_t byte[ITEMS];
     int pos[ITEMS], c[ITEMS], entry[ITEMS], row[ITEMS];
@@ -755,7 +758,7 @@ __global__ __launch_bounds__(THREADS) void read_kernel(const ReadParams p) {
     char* const out = side.out + static_cast<int64_t>(unit) * p.max_k * (side.chunks * 16);
 #pragma unroll
     for (int j = 0; j < ITEMS; ++j) {
-        if (pos[j] >= p.max_k) continue;
+        if (pos[j] >= rows_out) continue;
         if constexpr (FOUR) {
             const uint32_t codes = x[j][0];
             const float s = scale_of(byte[j]);
@@ -769,8 +772,9 @@ __global__ __launch_bounds__(THREADS) void read_kernel(const ReadParams p) {
 
 }  // namespace
 
-hipError_t launch_read(const kmi_paged_cache& c, void* k, void* v, int64_t max_k, hipStream_t stream) {
+hipError_t launch_read(const kmi_paged_cache& c, void* k, void* v, int64_t max_k, bool end, hipStream_t stream) {
     ReadParams p{};
+    p.end = end;
     p.c = device_cache(c);
     p.max_k = static_cast<int>(max_k);
     for (int w = 0; w < 2; ++w) {
@@ -831,5 +835,5 @@ extern "C" int kmi_paged_read(const kmi_paged_cache* c, void* k_out, void* v_out
         return fail(KMI_EINVAL, "kmi_paged_read: k_out and v_out must be 16-byte aligned and not null");
     if (max_k < 0 || !paged::read_fits(*c, max_k)) return fail(KMI_EINVAL, "kmi_paged_read: max_k out of range");
     if (max_k == 0 || c->batch == 0) return KMI_OK;
-    return hip_status(paged::launch_read(*c, k_out, v_out, max_k, static_cast<hipStream_t>(stream)), "kmi_paged_read");
+    return hip_status(paged::launch_read(*c, k_out, v_out, max_k, true, static_cast<hipStream_t>(stream)), "kmi_paged_read");
 }

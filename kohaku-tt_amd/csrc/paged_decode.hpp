@@ -10,8 +10,8 @@
 // tile's softmax and PV.  S^T = K Q^T leaves a query row per lane, its softmax state is scalar; P
 // feeds O^T += V^T P^T as it stands, in two 16-bit parts (a second product, hidden behind the
 // loads: 64 sequences x 2 heads x 8192 keys x 128 100.2 against 100.4 us, in 4 bits 35.5 against
-// 35.1, when both took that long), so that results are as close to 64-bit ones as their own rounding (0.0017 relative where
-// one part gave 0.0023).
+// 35.1, when both took that long), so that results are as close to 64-bit ones as their own
+// rounding (0.0017 relative where one part gave 0.0023).
 //
 // 16-bit caches: 16x16x32 MFMAs.  4-bit caches: the codes of K are the operand of the scaled
 // 16x16x128 MFMA as they lie in memory, with the cache's own scale bytes; no key is ever
@@ -20,8 +20,8 @@
 // exactly (elements below 2^-13 of the row's largest to within 2^-17 of it), fp16's eleven fit
 // three.  V's codes are widened by the packed conversions on their way into the LDS tile.
 //
-// Measured: that 16-bit call takes 85 us with its merge, 6.3 TB/s (a copy moves 5.13, the dense
-// decode kernel takes 97 us), the 4-bit one (143 MB) 31.8, 4.5 TB/s, and 54.5 with twice the
+// Measured: that 16-bit call takes 84 us with its merge, 6.4 TB/s (a copy moves 5.13, the dense
+// decode kernel takes 97 us), the 4-bit one (143 MB) 30.6, 4.7 TB/s, and 54.5 with twice the
 // sequences, 5.2: start, first latencies and the merge are fixed.  What made it so, in 4 bits: entries and lengths read
 // side by side, table entries clamped and scale bytes widened where they are used (a widening left
 // where the byte was loaded waited for the whole next tile: 38.4 -> 35.5 us), ranges computed and

@@ -522,6 +522,24 @@ def test_many_sequences(ops, dev, count):
 
 
 @pytest.mark.parametrize("bits", [16, 4])
+def test_workspaces_full_of_nan(ops, dev, bits):
+    """What a workspace held before is never read: partial rows of empty splits, the rows past a
+    sequence's length in the copy of a 4-bit cache."""
+    for new, before, at in (([1, 1], [5000, 3], {}), ([90, 40], [4000, 0], {}), ([200, 3], [10, 50], {"max_k": 9000})):
+        c = P.Cache([a + b for a, b in zip(new, before)], 2, 64, 64, 16, BF, bits)
+        held = c.to(dev)
+        q = _randn(sum(new), 8, 64, seed=2, dtype=BF).to(dev)
+        cu = torch.tensor(P.cu_of(new), dtype=torch.int32, device=dev)
+        args = {"cu_seq_q": cu, "max_q": max(new), "max_k": max(c.lens), **at}
+        torch.cuda.empty_cache()
+        spoilt = [torch.full((2**n,), math.nan, device=dev) for n in range(8, 25)]
+        torch.cuda.synchronize()
+        del spoilt
+        out = ops.sdpa_paged(q, **held, **args)
+        _check_attention(out, None, c, q.cpu(), P.cu_of(new), True, 0.125, bits == 4 and max(new) * 4 <= 32, BF)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
 def test_sequences_that_share_pages(ops, dev, bits):
     """A common prefix held once: each sequence reads it as its own, bit for bit."""
     c = P.Cache([96, 96, 96], 2, 64, 64, 16, BF, bits)
