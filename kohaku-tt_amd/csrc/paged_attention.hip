@@ -60,6 +60,39 @@ const char* check_attn(const kmi_paged_attn_args* a) {
     return nullptr;
 }
 
+// Splits of a decode call over a 16-bit cache: the fewest that keep CUs and wavefronts 85% at work, else
+// those that come nearest.  The cache's bytes bound such a call, and a CU with one workgroup more than
+// the others, or a wavefront with one tile more, is its end.  Measured (us, in brackets as many splits
+// as make two workgroups a CU, rounded up), heads of 128 dims: 48 units (sequences x K/V heads) of 8192
+// keys 37.2 (46.6), 80 59.6 (70.8), 24 24.3 (28.8), 16 17.8 (19.6), 128 85.7 (87.0), 250 157 (167), 28
+// of 16384 42.7 (53.3), 160 of 4096 57.9 (62.2), 200 77.2 (82.2), 32 17.0 (18.5), 300 of 2048 59.0
+// (62.6), 64 16.7 (18.6), 128 of 1024 16.5 (18.1).
+int64_t even_splits(int64_t units, int64_t keys, int64_t most) {
+    // How much of `slots` is at work while n things take them in rounds.
+    const auto share = [](int64_t n, int64_t slots) {
+        return n == 0 ? 0. : static_cast<double>(n) / static_cast<double>(slots * ceil_div(n, slots));
+    };
+    int64_t best = 1;
+    double fullest = 0.;
+    for (int64_t s = 1; s <= std::min<int64_t>(most, kMaxSplits); ++s) {
+        const double full = share(units * s, 256) * share(ceil_div(keys, kDecodeTile), 4 * s);
+        if (full > fullest) {
+            best = s;
+            fullest = full;
+        }
+        if (full >= 0.85) break;
+    }
+    return best;
+}
+
+// Over a 4-bit cache, whose tiles are small: as near to two workgroups a CU as splits come (us at that,
+// at even_splits' where that is another): 48 units of 8192 keys 20.2, 21.6, 80 23.9, 31.7, 24 15.1,
+// 15.6, 128 34.5, 43.8, 28 of 16384 21, 26, 160 of 4096 23.5 both, 200 28.4, 28.5, 300 of 2048 23.0,
+// 26.0.
+int64_t four_bit_splits(int64_t units, int64_t most) {
+    return std::min(std::max<int64_t>(1, (512 + units / 2) / std::max<int64_t>(1, units)), most);
+}
+
 Plan make_plan(const kmi_paged_attn_args* a) {
     Plan pl{};
     pl.dp = pad_dim(a);
@@ -71,17 +104,13 @@ Plan make_plan(const kmi_paged_attn_args* a) {
         pl.decode = true;
         pl.rows = vrows <= 16 ? 16 : 32;
         pl.nx = 1;
-        // Two workgroups of four wavefronts per CU, a tile for each of a split's wavefronts and
-        // two where there are many splits (us in a graph at 4, 7 / 20, 40 splits: 14/2 heads x 777
-        // keys x 64 8.1, 6.6; 4 bits, 3 x 4 tokens over 5001 keys 11.7, 12.3; 64 sequences x 2
-        // heads x 8192 keys x 128, at 2, 4, 6, 8 splits 100, 101, 103, 103, in 4 bits 52.5, 39.1,
-        // 38.9, 44.4).
         pl.min_split = kDecodeTile;
-        splits = std::min(ceil_div(512, std::max<int64_t>(1, units)),
-                          std::max(std::min<int64_t>(ceil_div(keys, 4 * kDecodeTile), 8), keys / (8 * kDecodeTile)));
+        // At most a tile for each of a split's wavefronts, two where there are many splits.
+        const int64_t most = std::max(std::min<int64_t>(ceil_div(keys, 4 * kDecodeTile), 8), keys / (8 * kDecodeTile));
+        splits = a->cache.bits == 4 ? four_bit_splits(units, most) : even_splits(units, keys, most);
         // Splits cost a second launch, 2.7 us of the GPU and 3 of the host; seven tiles a
         // wavefront at head dim 64, the time of three and a half at 128, cost less in one (777
-        // keys as above: 7.3 us in a graph, but 8 against 11 from the host).
+        // keys of 14/2 heads x 64: 7.3 us in a graph, 6.6 in seven, but from the host 8 against 11).
         if (ceil_div(keys, 4 * kDecodeTile) * pl.dp <= 7 * 64) splits = 1;
     } else {
         // Row tiles of the call, from its tokens (a tile begun per unit counts half).

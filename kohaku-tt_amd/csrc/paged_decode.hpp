@@ -20,7 +20,7 @@
 // exactly (elements below 2^-13 of the row's largest to within 2^-17 of it), fp16's eleven fit
 // three.  V's codes are widened by the packed conversions on their way into the LDS tile.
 //
-// Measured: that 16-bit call takes 84 us with its merge, 6.4 TB/s (a copy moves 5.13, the dense
+// Measured: that 16-bit call takes 83 us with its merge, 6.5 TB/s (a copy moves 5.13, the dense
 // decode kernel takes 97 us), the 4-bit one (143 MB) 30.6, 4.7 TB/s, and 54.5 with twice the
 // sequences, 5.2: start, first latencies and the merge are fixed.  What made it so, in 4 bits: entries and lengths read
 // side by side, table entries clamped and scale bytes widened where they are used (a widening left
