@@ -119,52 +119,49 @@ Plan make_plan(const kmi_paged_attn_args* a) {
                             ceil_div(a->cache.tokens * G, rows) * a->cache.heads_kv + units / 2);
         };
         const int64_t t4 = tiles(128), t2 = std::max<int64_t>(1, tiles(64));
-        // 128-row workgroups where they fill two thirds of the chip (two a CU; one past head dim 128,
-        // of 64 rows).  Prompts from their start do not pay for a merge and take 64 rows below a full
-        // chip.  Over longer keys splits fill it, of 128 rows unless those are few: seven eighths of a
-        // round or more than one and a half, for one whole round's workgroups all end together.
-        // Measured (us, 64 rows at 1, 2, 4, 8 splits / 128 rows at 1, 2, 3, 4, 5, 8):
-        //   4 x up to 1024 tokens of 32/8 heads over 8192 keys x 128 (744 tiles of 128) 384, 437,
-        //     472, 577 / 335, 353, 358, 371, 392
-        //   5 x 600 of 16/8 over 2100 x 128 (400) / 77, 96, 103, 113, 122, 151, over 8600 252, 269, ..
-        //   4 x 700 of 16/8 over 3700 (352) / 114, 122, 122, 130, 135, 160
-        //   5 x 500 of 16/8 over 3500 (320) / 108, 114, 110, 117, .., over 12500 356, 337, 299, 305, 319
-        //   8 ragged x 16/2 over up to 7000 (286) 111, 97, 114, 153 / 153, 98, .., 94, .., 119
-        //   6 x 400 of 14/2 over 3400 x 64 (264) / 80, 78, 68, 74, 74, 84
-        //   1 x 1024 of 32/8 over 2048 (256) / 56, 52, 61, 64, 66, 86
-        //   3 x 640 of 16/8 over 8640 (240) / 247, 215, 188, 191, 190, 202
-        //   2 x 777 of 16/8 over 4500, 4 bits (200) 90, 101, 106, 126 / 113, 84, 97, 94, 96
-        //   1 x 700 of 32/8 over 8700 (176) / 192, 138, 156, 139, 135, 140, over 30700 664, 439, .., 401
-        //   2 x 300 of 32/8 over 8300 (160) / 185, 132, 148, 125, 120, 132
-        //   2 x 400 of 14/2 over 3400 x 64 (88) / 64, 39, 36, 32, 30, 35
-        //   512 of 16/2 over 4600 (64) / 105, 62, 49, 43, 48, 43
-        //   512 of 14/2 over 8192 x 64 (56) 84, 50, 37, 43 / 134, 75, .., 44, .., 35
-        //   3 x 100 of 16/2 over 9100 (42; 78 of 64) at 1 .. 6, 8 splits 141, 78, 66, 54, 47, 66, 55 /
-        //   8 x 32 of 16/2 over 8224 (64 of 64) 128, 72, 46, 41, 4 x 64 over 4160 68, 41, 28, 27, 16 x 16
-        //     over 2064 38, 26, 20, 22 /
-        //   prompts: 2048 of 14/2 x 64 (224) 26, 39, 42, 42 / 38, 38, .., 39; 2 x 700 of 16/2 x 128
-        //     (176) 20, 33, 33, 33 / 23, 36, .., 35; 4 x 2048 of 32/8 x 128 231, 366, .. / 197, 323, ..;
-        //     512 of 14/2 x 64 (56 of 64 rows) 10.0 whole, 13.2 in two
+        // 128-row workgroups where they fill two thirds of the chip (two a CU, of which head dim 64 takes
+        // twice as many; one past 128, of 64 rows).  Prompts from their start do not pay for a merge and take 64
+        // rows below a full chip.  Over longer keys splits fill it, of 128 rows unless those are few:
+        // as many as make one round, or, where that leaves a quarter of it idle, a round and a half.
+        // Measured (us, tiles, whole and in 2, 3, 4, 5, 6, 8, 12 splits; * as planned):
+        //   128 rows, head dim 128: 4 x up to 1024 tokens of 32/8 heads over 8192 keys (744) 335*, 353,
+        //     358, 371; 5 x 600 of 16/8 over 2100 (400) 70*, 87, 95; 4 x 700 over 3700 (352) 114*, 127,
+        //     125; 5 x 500 over 3500 (320) 109, 121, 112*, 118, over 12500 361, 340, 303*, 308; 1 x 1024 of
+        //     32/8 over 2048 (256) 56, 53*, 64; 3 x 640 of 16/8 over 8640 (240) 195, 162*, 184, 174, 186;
+        //     2 x 777 of 16/8 over 4500 (208) 107, 84*, 105, 97; 1 x 700 of 32/8 over 8700 (176) 195,
+        //     139, 160, 143, 137*, 146, over 30700 672, 444, 516, 439, 405*, 427, 400; 2 x 300 of 32/8
+        //     over 8300 (160) 186, 133, 105*, 129, 123; 512 of 16/2 over 4600 (64) 106, 63, 49, 44, 48, 44,
+        //     44*, 53; 256 of 32/8 over 30256 (64) 657, 339, 233, 182, 188, 172, 154*, 177
+        //   of head dim 64: 9 x 500 of 14/2 over 3500 (504) 126, 96*, 111, 107; 6 x 400 over 3400 (264) 78,
+        //     73, 67*, 71; 2 x 400 over 3400 (88) 63, 38, 35, 33, 29*, 37, 35, 40
+        //   64 rows: 3 x 100 of 16/2 x 128 over 9100 (78) 139, 77, 57, 54, 47, 44*, 58, 52; 8 x 32 over
+        //     8224 (64) 127, 71, 53, 45, 46, 43, 40*, 50; 4 x 64 over 4160 (64) 68, 41, 33, 29, 30, 28,
+        //     27*, 34; 16 x 16 over 2064 (64) 37, 26, 22, 20*, 22, 22, 23, 29; 300 of 16/2 x 256 over 4300
+        //     (76) 107, 65, 51*, 75; 4 x 200 of 16/4 x 192 over 2200 (208) 54*, 67
+        //   prompts (64 rows / 128 rows, whole and in 2, 4, 8): 2048 of 14/2 x 64 (224 of 128) 26, 39, 42,
+        //     42 / 38, 38, 39, 39; 2 x 700 of 16/2 x 128 (176) 20, 33, 33, 33 / 23, 36, 35, 35; 4 x 2048
+        //     of 32/8 x 128 231, 366, .. / 197, 323, ..; 512 of 14/2 x 64 (56 of 64 rows) 10.0, 13.2
         const bool own = a->causal && 2 * a->max_q > keys;
-        // (Past head dim 128, one a CU: 300 tokens of 16/2 x 256 over 4300, 76 tiles, at 1, 2, 3, 4 splits
-        // 107, 64, 51, 74; 4 x 200 of 16/4 x 192 over 2200, 208 tiles, 54, 68.)
-        const int64_t slots = pl.dp <= 128 ? 512 : 256, room = pl.dp <= 128 ? 448 : 240;
+        const int64_t slots = pl.dp <= 128 ? 512 : 256;
         pl.row_groups = 2;
         pl.min_split = 256;
-        splits = std::max<int64_t>(1, std::min(room / t2, std::max(keys / 512, slots / 2 / t2)));
-        if (pl.dp <= 128 && t4 >= (own ? room : slots * 2 / 3)) {
-            pl.row_groups = 4;
-            splits = 1;
-        } else if (own) {
+        splits = std::min(slots / t2, std::max(keys / 512, slots / 2 / t2));
+        if (own) {
             splits = t2 >= slots / 8 ? 1 : slots / 4 / t2;
+            if (pl.dp <= 128 && t4 >= 448) {
+                pl.row_groups = 4;
+                splits = 1;
+            }
         } else if (pl.dp <= 128 && t4 >= 48) {
             pl.row_groups = 4;
-            const int64_t many = (840 + t4 / 2) / t4;
-            if (t4 >= 128 && keys >= 1600 * many)
-                splits = many;
-            else
-                splits = t4 >= 216 ? (keys >= 3000 ? 3 : 2) : room / t4;
+            const int64_t more = (840 + t4 / 2) / t4;  // a round and a half
+            splits = slots / t4;
+            if (pl.dp <= 64)
+                splits = std::max(splits, std::min(2 * slots / t4, keys / 1000));
+            else if (t4 < slots * 2 / 3 && splits * t4 < slots * 3 / 4 && keys >= 1000 * more)
+                splits = more;
         }
+        splits = std::max<int64_t>(1, splits);
         pl.rows = 32 * pl.row_groups;
         pl.nx = static_cast<int>(ceil_div(vrows, pl.rows));
     }

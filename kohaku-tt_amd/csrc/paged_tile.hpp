@@ -32,12 +32,13 @@ __device__ __forceinline__ int sorted_sequence(const paged::AttnParams& p, int n
     return __builtin_amdgcn_readfirstlane(found ? __builtin_ctzll(found) : 0);
 }
 
-// Workgroup order.  Row tiles of a unit (sequence, K/V head) read the same keys, so `group` of them
-// lie on one XCD (block b runs on XCD b % 8) next to each other and share its L2; groups go round the
-// XCDs there and back, those with most keys first: the longest sequence's heads, then the next
-// one's; where a causal call's keys are mostly its own queries (prompts from their start) the last
-// row tiles of every unit, then those before them.  The last workgroups zero the rows behind the last
-// sequence.
+// Workgroup order.  Row tiles of a unit (sequence, K/V head) read the same keys of a split, so a group
+// of them lies on one XCD (block b runs on XCD b % 8), its tiles next to each other, and shares its L2.
+// Groups of one size go round the XCDs there and back, each split's on its own (a unit's splits
+// together on one XCD left others idle: 3 x 640 tokens of 16/8 heads over 8640 keys x 128 215 us, so
+// 162), those with most keys first: the longest sequence's heads, then the next one's; where a causal
+// call's keys are mostly its own queries (prompts from their start) the last row tiles of every unit,
+// then those before them.  The last workgroups zero the rows behind the last sequence.
 template <typename T, int DP, int RG>
 __global__ __launch_bounds__(NTHREADS, tile_waves(DP)) void paged_attn_tile_kernel(const paged::AttnParams p) {
     constexpr size_t TILES = 4 * sizeof(T) * Tile<T, DP, tile_keys(DP, RG)>::ELEMS;
@@ -47,13 +48,14 @@ __global__ __launch_bounds__(NTHREADS, tile_waves(DP)) void paged_attn_tile_kern
         paged::zero_tail<T>(p, gridDim.x - 1 - lin);
         return;
     }
-    const int x = lin & 7, s = lin >> 3, per = p.tile_group * p.splits;
-    const int round = s / per, i = s - round * per;
-    const int g = 8 * round + (round & 1 ? 7 - x : x);
-    const int units = p.batch * p.hkv;
-    const int unit = p.rows_first ? g % units : g / p.tile_groups, xg = p.rows_first ? g / units : g - unit * p.tile_groups;
-    const int split = i / p.tile_group, xi = xg * p.tile_group + (i - split * p.tile_group);
-    if (unit >= units || xi >= p.nx) return;
+    const int x = lin & 7, s = lin >> 3;
+    const int round = s / p.tile_group, i = s - round * p.tile_group;
+    const int item = 8 * round + (round & 1 ? 7 - x : x);
+    const int units = p.batch * p.hkv, parts = p.tile_groups * p.splits;
+    const int unit = p.rows_first ? item % units : item / parts, part = p.rows_first ? item / units : item - unit * parts;
+    const int xg = fdiv(part, p.fd_splits), split = part - xg * p.splits;
+    const int xi = xg * p.tile_group + i;
+    if (unit >= units || part >= parts || xi >= p.nx) return;
     int bh = unit;
     if (p.sorted) {
         const int nth = fdiv(unit, p.fd_hkv);
@@ -78,9 +80,10 @@ hipError_t launch_tile(const AttnParams& p_in, int rg, hipStream_t stream) {
         p.tile_group /= 2;
     p.rows_first = p.causal && 2 * static_cast<int64_t>(p.seq_q) > p.c.capacity;
     p.tile_groups = (p.nx + p.tile_group - 1) / p.tile_group;
+    p.tile_group = (p.nx + p.tile_groups - 1) / p.tile_groups;  // (of one size)
     p.sorted = p.batch > 1 && p.batch <= 64 && static_cast<int64_t>(units) * p.nx * p.splits > 256;
-    const int rounds = (units * p.tile_groups + 7) / 8;
-    const dim3 grid(static_cast<unsigned>(8 * rounds * p.tile_group * p.splits + p.tail_blocks));
+    const int rounds = (units * p.tile_groups * p.splits + 7) / 8;
+    const dim3 grid(static_cast<unsigned>(8 * rounds * p.tile_group + p.tail_blocks));
     if constexpr (DP <= 128) {
         if (rg == 4) {
             hipLaunchKernelGGL((fwd::paged_attn_tile_kernel<T, DP, 4>), grid, dim3(fwd::NTHREADS), 0, stream, p);
