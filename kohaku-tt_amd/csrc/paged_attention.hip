@@ -107,11 +107,13 @@ Plan make_plan(const kmi_paged_attn_args* a) {
         pl.min_split = kDecodeTile;
         // At most a tile for each of a split's wavefronts, two where there are many splits.
         const int64_t most = std::max(std::min<int64_t>(ceil_div(keys, 4 * kDecodeTile), 8), keys / (8 * kDecodeTile));
-        splits = a->cache.bits == 4 ? four_bit_splits(units, most) : even_splits(units, keys, most);
         // Splits cost a second launch, 2.7 us of the GPU and 3 of the host; seven tiles a
         // wavefront at head dim 64, the time of three and a half at 128, cost less in one (777
         // keys of 14/2 heads x 64: 7.3 us in a graph, 6.6 in seven, but from the host 8 against 11).
-        if (ceil_div(keys, 4 * kDecodeTile) * pl.dp <= 7 * 64) splits = 1;
+        if (ceil_div(keys, 4 * kDecodeTile) * pl.dp <= 7 * 64)
+            splits = 1;
+        else
+            splits = a->cache.bits == 4 ? four_bit_splits(units, most) : even_splits(units, keys, most);
     } else {
         // Row tiles of the call, from its tokens (a tile begun per unit counts half).
         const auto tiles = [&](int64_t rows) {

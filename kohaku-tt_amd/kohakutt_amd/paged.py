@@ -192,8 +192,9 @@ def sdpa_paged(q, k_cache, v_cache, block_table, key_lengths, cu_seq_q=None, max
 
     `max_q` (1 without `cu_seq_q`, else T unless given) must cover every sequence's queries:
     rows past it hold unspecified values.  `max_k` bounds the keys: those past it are not read
-    (by default every key that `block_table` can name, which sizes a launch for that many, so
-    give the batch's longest length where it is known).  No gradient."""
+    (by default every key that `block_table` can name, which sizes a launch for that many and, over
+    a 4-bit cache with more than 32 query rows per cache head, a 16-bit copy of them, so give the
+    batch's longest length where it is known).  No gradient."""
     return _SDPA(q, k_cache, v_cache, block_table, key_lengths, cu_seq_q, max_q, max_k, is_causal,
                  scale, False, k_scale, v_scale)[0]
 
