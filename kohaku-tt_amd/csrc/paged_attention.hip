@@ -364,7 +364,6 @@ extern "C" int kmi_paged_attn(const kmi_paged_attn_args* a, void* workspace, siz
     p.tail_blocks = tail_blocks(a);
     p.rows_total = a->cache.tokens;
     p.fd_splits = fwd::fast_div(static_cast<uint32_t>(p.splits));
-    p.fd_units = fwd::fast_div(static_cast<uint32_t>(p.batch * p.hkv));
     p.fd_hkv = fwd::fast_div(static_cast<uint32_t>(p.hkv));
     p.fd_group = fwd::fast_div(static_cast<uint32_t>(p.group));
     if (pl.splits > 1) {

@@ -125,11 +125,12 @@ struct Held {
 };
 
 // The places of a workgroup's tokens and, for rotated calls, their angles' cosines and sines (F:
-// float, or double, then in both), into LDS.  Tokens of one sequence (nearly every workgroup's) find it by scalar
-// loads, which do not queue behind the vectors in flight, and wait for one vector load, the
-// table's; a workgroup across sequences searches per token.
+// float, or double, then in both), into LDS.  Tokens of one sequence (nearly every workgroup's) find
+// it by scalar loads, which do not queue behind the vectors in flight, and wait for one vector load,
+// the table's; a workgroup across sequences searches per token.
 template <typename F>
-__device__ __forceinline__ void place_tokens(const AppendParams& p, const int64_t (&st)[3], const int64_t (&ss)[3], int t0, int nt, Held* held, float* cosine,
+__device__ __forceinline__ void place_tokens(const AppendParams& p, const int64_t (&st)[3], const int64_t (&ss)[3],
+                                             int t0, int nt, Held* held, float* cosine,
                                              float* sine, F* cosine_f = nullptr, F* sine_f = nullptr) {
     const Cache& c = p.c;
     const int half = cosine ? p.rd / 2 : 0;
@@ -372,15 +373,14 @@ __device__ __forceinline__ int max_of_four(int v) {
     return max(v, __builtin_amdgcn_mov_dpp(v, 0x4e, 0xf, 0xf, true));  // lanes 2, 3, 0, 1
 }
 
-// The group's scale byte and exponent e from the largest exponent field (biased by `bias`,
-// `top_field` for infinities and NaN) of its values.
+// The group's scale byte and exponent e from the largest exponent field of its 64-bit values.
 struct Scale {
     int byte, e;
 };
-__device__ __forceinline__ Scale group_scale(int field, int bias, int top_field) {
+__device__ __forceinline__ Scale group_scale(int field) {
     field = max_of_four(field);
-    const int e = field == 0 ? -127 : min(max(field - bias - 2, -126), 127);
-    return Scale{field == top_field ? 255 : e + 127, e};
+    const int e = field == 0 ? -127 : min(max(field - 1025, -126), 127);
+    return Scale{field == 0x7ff ? 255 : e + 127, e};
 }
 
 // Eight values over a power of two as codes: nearest, ties to even, saturating.
@@ -595,7 +595,7 @@ __global__ __launch_bounds__(THREADS) void append4_kernel(const AppendParams p) 
             int top = 0;
 #pragma unroll
             for (int e = 0; e < 8; ++e) top = max(top, static_cast<int>(__double2hiint(y[e]) & 0x7fffffff));
-            const Scale scale = group_scale(top >> 20, 1023, 0x7ff);
+            const Scale scale = group_scale(top >> 20);
             const double inv = __hiloint2double((1023 - scale.e) << 20, 0);
             float f[8];
 #pragma unroll
