@@ -733,6 +733,34 @@ def test_serving_run_and_graph(ops, dev, bits):
         check(k, v, qr, out, None)
 
 
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("d,rows", [(256, 1), (256, 5), (192, 1), (96, 3), (256, 40), (128, 150)])
+def test_captured_attention(ops, dev, bits, d, rows):
+    """Every kind of kernel in a graph (those with more than 64 KB of LDS among them), replayed while
+    lengths and queries change."""
+    lens = [700, 300, rows]
+    c = P.Cache(lens, 2, d, d, 32, BF, bits)
+    held = c.to(dev)
+    q = torch.zeros(3 * rows, 8, d, dtype=BF, device=dev)
+    cu = torch.arange(0, 3 * rows + 1, rows, dtype=torch.int32, device=dev)
+    args = {**held, "cu_seq_q": cu, "max_q": rows, "max_k": 700}
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        ops.sdpa_paged(q, **args)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.sdpa_paged(q, **args)
+    for seed in range(3):
+        q.copy_(_randn(3 * rows, 8, d, seed=seed, dtype=BF))
+        held["key_lengths"].copy_(torch.tensor([700 - 100 * seed, 300 - seed, rows], dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ops.sdpa_paged(q, **args))
+        c.lens = held["key_lengths"].tolist()
+        _check_attention(out, None, c, q.cpu(), list(range(0, 3 * rows + 1, rows)), True, d**-0.5, bits == 4 and rows * 4 <= 32, BF)
+
+
 def test_two_streams_at_once(ops, dev):
     """Calls in flight on two streams keep their own workspaces."""
     c = [P.Cache([3000, 2000], 1, 64, 64, 16, BF, 16, seed=s) for s in (0, 1)]
